@@ -53,8 +53,15 @@ typedef enum h3_dtype {
     H3_BF16 = 0,
     H3_F32 = 1,
     H3_F64 = 2,
-    H3_I64 = 3
+    H3_I64 = 3,
+    H3_U8 = 4   /* bytes: codes and scales of 4-bit matrices, nothing else */
 } h3_dtype;
+
+/* Microscaled 4-bit formats: blocks of consecutive columns of e2m1 codes share a scale. */
+typedef enum h3_fp4_format {
+    H3_MXFP4 = 0,   /* blocks of 32, scale 2^(byte - 127); the tensor scale is 1 */
+    H3_NVFP4 = 1    /* blocks of 16, unsigned e4m3 scale times the tensor scale, a power of two in [2^-64, 2^64] */
+} h3_fp4_format;
 
 typedef enum h3_status {
     H3_OK = 0,
@@ -287,6 +294,43 @@ int h3_pack_gate_up(const h3_tensor *dst, const h3_tensor *src, void *stream);
  * bitwise the same columns.  K a multiple of 8, rows 16-byte aligned. */
 int h3_adaln_projection(const h3_tensor *y, const h3_tensor *x, const h3_tensor *w, const h3_tensor *bias,
                         void *stream);
+
+/* ---------------- microscaled 4-bit projections ---------------- */
+
+/* A 4-bit matrix [rows, cols] is two byte tensors (no counterpart in the reference):
+ *   codes  [rows, ceil(cols/32)*16], inner stride 1, rows 16-byte aligned: column 2i in
+ *          the low nibble of byte i, 2i+1 in the high one, zero codes past cols;
+ *   scales [ceil(rows/128), ceil(blocks/4), 512] contiguous, 16-byte aligned, blocks =
+ *          ceil(cols / block size): the scale of row r, block b is byte
+ *          (r%32)*16 + (r%128)/32*4 + b%4 of chunk [r/128][b/4].  Blocks past the last
+ *          hold 0; rows past the last one may hold anything. */
+
+/* codes, scales = x [rows, cols] BF16 (inner stride 1) in `format`.
+ *   MXFP4: scale 2^e, e = clamp(floor(log2 amax) - 2, -127, 127)
+ *   NVFP4: scale s * tensor_scale, s = e4m3(amax / (6 * tensor_scale)), nearest-even, at most 448
+ * and codes e2m1(x / scale), nearest-even, at most 6 in magnitude.  A block with an
+ * infinity or a NaN gets the NaN scale (255, 127); one whose scale rounds to 0 zero codes. */
+int h3_quantize_fp4(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int32_t format,
+                    float tensor_scale, void *stream);
+
+/* y [rows, cols] BF16 = the values the codes and scales stand for (exact: at most 6
+ * significant bits). */
+int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tensor *scales, int32_t format,
+                      float tensor_scale, void *stream);
+
+/* y [M,N] = bf16(xq wq^T + bias): x [M,K] BF16 is quantised into x_codes / x_scales
+ * (caller-owned workspace of x's 4-bit shapes, any contents) and multiplied with the
+ * 4-bit weight [N,K] of the same format; fp32 accumulation, one rounding.  bias [N] BF16
+ * or NULL.  Any M, N, K >= 1 (K at most 2^24); rows of y and x contiguous. */
+int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *x_codes, const h3_tensor *x_scales,
+                  const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int32_t format,
+                  float x_tensor_scale, float w_tensor_scale, void *stream);
+
+/* h3_linear_fp4 for x that is in 4 bits already (several projections of the same rows);
+ * cols = K. */
+int h3_linear_fp4_quantized(const h3_tensor *y, const h3_tensor *x_codes, const h3_tensor *x_scales,
+                            const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int64_t cols,
+                            int32_t format, float x_tensor_scale, float w_tensor_scale, void *stream);
 
 /* ---------------- model wrapper ops (outside the block loop) ---------------- */
 

@@ -6,9 +6,10 @@ pointwise ops, mha, linear, and the fp32 linear / row gather / SiLU ops of the
 model wrapper); ``block`` composes one DiT block, ``step`` the 40-block
 denoising step, ``model`` the whole transformer forward around it (input
 projections, token refiner, packing, output norm and projections);
-``ulysses`` shards the block over GPUs with the head<->sequence all-to-all.
+``fp4`` holds the microscaled 4-bit matrices and projections; ``ulysses`` shards the block over GPUs with the head<->sequence all-to-all.
 """
-from . import ops  # noqa: F401
+from . import fp4, ops  # noqa: F401
+from .fp4 import *  # noqa: F401,F403
 from .ops import *  # noqa: F401,F403
 from ._lib import library_path, load  # noqa: F401
 

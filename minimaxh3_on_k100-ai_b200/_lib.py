@@ -26,7 +26,7 @@ _STATUS = {
     9: "row index outside the indexed tensor",
     10: "request exceeds the library's static scratch capacity",
 }
-_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float64: 2, torch.int64: 3}
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float64: 2, torch.int64: 3, torch.uint8: 4}
 
 
 class H3Tensor(ctypes.Structure):
@@ -76,6 +76,10 @@ SIGNATURES = {
     "h3_linear_gated_residual_rms_modulate_noalloc": [P, P, P, P, P, P, P, P, P, _F, _V],
     "h3_pack_gate_up": [P, P, _V],
     "h3_linear_qkv_norm_rope": [P, P, P, P, P, _I, P, P, P, P, _F, _V],
+    "h3_quantize_fp4": [P, P, P, _I, _F, _V],
+    "h3_dequantize_fp4": [P, P, P, _I, _F, _V],
+    "h3_linear_fp4": [P, P, P, P, P, P, P, _I, _F, _F, _V],
+    "h3_linear_fp4_quantized": [P, P, P, P, P, P, ctypes.c_int64, _I, _F, _F, _V],
     "h3_linear_f32": [P, P, P, P, _V],
     "h3_gather_rows": [P, P, P, _V],
     "h3_index_copy_rows": [P, P, P, _V],

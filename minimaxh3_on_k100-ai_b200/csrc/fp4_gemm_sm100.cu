@@ -1,0 +1,369 @@
+// Projections with microscaled 4-bit operands on tcgen05's block-scaled MMA (sm_100a):
+//
+//   y[m][n] = bf16( t * sum_k xq[m][k] wq[n][k] + bias[n] ),   fp32 accumulation,
+//
+// xq and wq in one format (layout: fp4_common.cuh), t the product of their tensor scales.
+// The tensor core multiplies the codes, applies both block scales and adds in fp32, so
+// nothing is widened in memory: a product reads K/2 + K/block bytes per row.
+//
+// swap form: the weight's rows are the M = 128 side of the MMA and BN rows of x the N
+// side, so a few tokens cost N = 16 columns, not a 128-row tile.  A CTA owns one tile; a
+// cluster of up to 8 CTAs splits K, each CTA leaves its fp32 tile in shared memory and
+// sums its share of the columns over the cluster in rank order (fixed order, no atomics,
+// no scratch in global memory).  Bound by reading the weights (HBM).
+#include <math.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "fp4_common.cuh"
+#include "h3_abi_util.h"
+#include "h3_common.cuh"
+#include "sm100_ptx.cuh"
+#include "tma_host.h"
+
+namespace h3 {
+namespace fp4 {
+
+int quantize(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int fmt, float tensor_scale,
+             cudaStream_t stream);
+
+constexpr int BK = 256;                          // columns per K tile: one 128-byte swizzle span
+constexpr int KSTEP = 64;                        // columns per MMA
+__host__ __device__ constexpr int tile_chunks(int fmt) { return fmt == MX ? 2 : 4; }   // scale chunks per K tile
+
+struct Params {
+    int M, N;                    // rows of x, rows of w
+    int ktiles, chunks, ksteps;  // along K: tiles, scale chunks, MMAs
+    const uint8_t *sx, *sw;      // scales
+    __nv_bfloat16 *y;
+    int64_t ldy;
+    const __nv_bfloat16 *bias;   // may be null
+    float t;
+    int num_m, num_n;            // tiles
+    int wide;                    // 4-column (8-byte) stores allowed
+    int dependent;               // launched behind the quantisation of x: only w may be read before it ends
+};
+
+template <int FMT, int BN>
+struct Swap {
+    static constexpr int CH = tile_chunks(FMT);
+    static constexpr int A_BYTES = 128 * 128;                 // 128 weight rows
+    static constexpr int B_BYTES = BN * 128;
+    static constexpr int SF_BYTES = CH * CHUNK;
+    static constexpr int STAGE = A_BYTES + B_BYTES + 2 * SF_BYTES;
+    static constexpr int STAGE_PAD = (STAGE + 1023) / 1024 * 1024;
+    static constexpr int BUDGET = 110 * 1024;                 // two CTAs per SM
+    static constexpr int STAGES = BUDGET / STAGE_PAD;
+    static constexpr int RED_BYTES = BN * 128 * 4;            // the fp32 tile, in the ring's place
+    static constexpr int OFF_BAR = STAGES * STAGE_PAD > RED_BYTES ? STAGES * STAGE_PAD : RED_BYTES;
+    static constexpr int SMEM = OFF_BAR + (2 * STAGES + 1) * 8 + 16 + 1024;
+    static constexpr int SF_COLS = CH * 4;                    // tensor memory columns of one operand's scales
+    static constexpr int SF_COL0 = BN < 32 ? 32 : BN;         // behind the accumulator
+    static constexpr uint32_t TMEM = SF_COL0 + 4 * SF_COLS <= 128 ? 128 : 256;
+    static_assert(SF_COL0 + 4 * SF_COLS <= (int)TMEM, "tensor memory");
+    static_assert(STAGES >= 3, "ring");
+};
+constexpr int SWAP_THREADS = 128;
+
+// 16 bytes from CTA `rank`'s shared memory at this CTA's address `addr`
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(a)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// grid: x = cluster rank (K share), y = weight row tile, z = x row tile
+template <int FMT, int BN>
+__global__ void __launch_bounds__(SWAP_THREADS)
+    swap_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, Params p) {
+    using C = Swap<FMT, BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
+    uint64_t *empty = full + C::STAGES;
+    uint64_t *done = empty + C::STAGES;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster spans grid x
+    const int n0 = (int)blockIdx.y * 128, m0 = (int)blockIdx.z * BN;
+    const int k_begin = (int)((int64_t)p.ktiles * rank / split), k_end = (int)((int64_t)p.ktiles * (rank + 1) / split);
+    const int nk = k_end - k_begin;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tx);
+        tma_prefetch_desc(&tw);
+        auto load_w = [&](int i) {
+            const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
+            uint8_t *st = smem + slot * C::STAGE_PAD;
+            mbar_expect_tx(&full[slot], C::A_BYTES + C::B_BYTES + 2 * ch * CHUNK);
+            tma_load_2d(st, &tw, &full[slot], kt * 128, n0);
+            bulk_load(st + C::A_BYTES + C::B_BYTES, p.sw + ((int64_t)blockIdx.y * p.chunks + kt * C::CH) * CHUNK,
+                      ch * CHUNK, &full[slot]);
+        };
+        auto load_x = [&](int i) {
+            const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
+            uint8_t *st = smem + slot * C::STAGE_PAD;
+            tma_load_2d(st + C::A_BYTES, &tx, &full[slot], kt * 128, m0);
+            bulk_load(st + C::A_BYTES + C::B_BYTES + C::SF_BYTES,
+                      p.sx + ((int64_t)(m0 >> 7) * p.chunks + kt * C::CH) * CHUNK, ch * CHUNK, &full[slot]);
+        };
+        // the weights do not wait for the quantisation of x: fill the ring with them first
+        const int head = min(nk, C::STAGES);
+        for (int i = 0; i < head; ++i) load_w(i);
+        if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int i = 0; i < head; ++i) load_x(i);
+        for (int i = head; i < nk; ++i) {
+            if (!mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, abort_flag)) break;
+            load_w(i);
+            load_x(i);
+        }
+    } else if (warp == 1 && lane == 0) {
+        const uint32_t base = smem_u32(smem);
+        bool ok = true;
+        for (int i = 0; i < nk; ++i) {
+            const int slot = i % C::STAGES, kt = k_begin + i;
+            ok = mbar_wait(&full[slot], (i / C::STAGES) & 1, abort_flag);
+            // two scale buffers: the MMAs of tile i - 2 must have read the one about to be overwritten
+            if (ok && i >= 2) ok = mbar_wait(&empty[(i - 2) % C::STAGES], ((i - 2) / C::STAGES) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sa = base + slot * C::STAGE_PAD, sb = sa + C::A_BYTES;
+            const uint32_t ssa = sb + C::B_BYTES, ssb = ssa + C::SF_BYTES;
+            const uint32_t ta = tmem + C::SF_COL0 + (i & 1) * 2 * C::SF_COLS, tb = ta + C::SF_COLS;
+            const int ch = min(C::CH, p.chunks - kt * C::CH);
+            for (int c = 0; c < ch; ++c) {
+                tmem_cp_scales<false>(ta + 4 * c, smem_desc_rows16(ssa + c * CHUNK));
+                tmem_cp_scales<false>(tb + 4 * c, smem_desc_rows16(ssb + c * CHUNK));
+            }
+            const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
+            const uint32_t tb0 = tb + ((m0 & 127) >> 5);     // this tile's rows within the 128-row chunk
+            for (int s = 0; s < steps; ++s) {
+                const int c = FMT == MX ? s >> 1 : s;
+                const uint32_t id = FMT == MX ? (s & 1) * 2 : 0;
+                umma_fp4<FMT == MX, false>(tmem, smem_desc_sw128(sa + s * 32, 16, 1024),
+                                           smem_desc_sw128(sb + s * 32, 16, 1024),
+                                           idesc_fp4(128, BN, FMT == MX, id), ta + 4 * c, tb0 + 4 * c,
+                                           (i > 0 || s > 0) ? 1u : 0u);
+            }
+            umma_commit(&empty[slot]);
+        }
+        if (ok) umma_commit(done);
+        else drain_in_flight();
+    }
+    __syncwarp();
+    const bool ok = nk == 0 || __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag));
+    tc_fence_after();
+    // lane = weight row: column c of the tile becomes 128 consecutive floats
+    const uint32_t red = smem_u32(smem);
+    if (ok) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < BN; c0 += 16) {
+            uint32_t v[16];
+            if (nk > 0) {
+                tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
+                tmem_ld_wait();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                st_shared_f32(red + ((c0 + i) * 128 + warp * 32 + lane) * 4, nk > 0 ? v[i] : 0u);
+        }
+    }
+    tc_fence_before();
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    if (ok) {
+        const int n = n0 + lane * 4;
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) b[e] = __bfloat162float(p.bias[n + e]);
+        }
+        const int cols = min(BN, p.M - m0);
+        for (int c = rank * 4 + warp; c < cols; c += split * 4) {
+            float4 acc = ld_cluster_f4(red + (c * 128 + lane * 4) * 4, 0);
+#pragma unroll 1
+            for (int r = 1; r < split; ++r) {
+                const float4 o = ld_cluster_f4(red + (c * 128 + lane * 4) * 4, (uint32_t)r);
+                acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+            }
+            const float f[4] = {fmaf(acc.x, p.t, b[0]), fmaf(acc.y, p.t, b[1]), fmaf(acc.z, p.t, b[2]),
+                                fmaf(acc.w, p.t, b[3])};
+            __nv_bfloat16 *dst = p.y + (int64_t)(m0 + c) * p.ldy + n;
+            if (p.wide && n + 4 <= p.N) {
+                *reinterpret_cast<uint2 *>(dst) = pack4(f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < p.N) dst[e] = __float2bfloat16_rn(f[e]);
+            }
+        }
+    }
+    if (split > 1) cluster_sync();   // no CTA leaves while another reads its tile
+    else __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM);
+    }
+}
+
+template <int FMT, int BN>
+int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    using C = Swap<FMT, BN>;
+    auto kernel = swap_kernel<FMT, BN>;
+    CUtensorMap tx, tw;
+    H3_CHECK(make_tmap_bytes(&tx, xc->data, xc->shape[1], xc->shape[0],
+                             xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, BN));
+    H3_CHECK(make_tmap_bytes(&tw, wc->data, wc->shape[1], wc->shape[0],
+                             wc->shape[0] > 1 ? wc->strides[0] : wc->shape[1], 128, 128));
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
+    if (!ready[dev].load()) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+            return H3_ERR_LAUNCH;
+        ready[dev].store(true);
+    }
+    p.num_m = (p.M + BN - 1) / BN;
+    p.num_n = (p.N + 127) / 128;
+    if (p.num_m > 65535 || p.num_n > 65535) return H3_ERR_UNSUPPORTED;
+    // K shares: as many as two CTAs per SM leave room for
+    const int64_t tiles = (int64_t)p.num_m * p.num_n, slots = 2 * num_sms();
+    int split = (int)(slots / tiles);
+    split = split < 1 ? 1 : split > 8 ? 8 : split;
+    if (split > p.ktiles) split = p.ktiles;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(split, p.num_n, p.num_m);
+    cfg.blockDim = dim3(SWAP_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.dependent ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, p) != cudaSuccess) {
+        cudaGetLastError();
+        return H3_ERR_LAUNCH;
+    }
+    return launch_status();
+}
+
+template <int FMT>
+int multiply(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    if (p.M <= 16) return launch_swap<FMT, 16>(xc, wc, p, stream);
+    if (p.M <= 32) return launch_swap<FMT, 32>(xc, wc, p, stream);
+    if (p.M <= 64) return launch_swap<FMT, 64>(xc, wc, p, stream);
+    return launch_swap<FMT, 128>(xc, wc, p, stream);
+}
+
+// Checks of y, bias and the operands' widths; fills everything but the tile counts.
+int check_product(const h3_tensor *y, const h3_tensor *xc, const h3_tensor *xs, const h3_tensor *wc,
+                  const h3_tensor *ws, const h3_tensor *bias, int64_t rows, int64_t cols, int fmt, float tx, float tw,
+                  Params *p) {
+    if (!wc) return H3_ERR_NULL;
+    H3_CHECK(check_bf16(y));
+    if (fmt != MX && fmt != NV) return H3_ERR_UNSUPPORTED;
+    if (cols < 1 || wc->ndim != 2) return H3_ERR_BAD_SHAPE;
+    const int64_t outs = wc->shape[0];
+    H3_CHECK(check_held(wc, ws, fmt, outs, cols));
+    H3_CHECK(check_held(xc, xs, fmt, rows, cols));
+    if (y->ndim != 2 || y->shape[0] != rows || y->shape[1] != outs) return H3_ERR_BAD_SHAPE;
+    if ((outs > 1 && y->strides[1] != 1) || (rows > 1 && y->strides[0] < outs)) return H3_ERR_BAD_LAYOUT;
+    if (bias) {
+        H3_CHECK(check_bf16(bias));
+        if (bias->ndim != 1 || bias->shape[0] != outs) return H3_ERR_BAD_SHAPE;
+        if (outs > 1 && bias->strides[0] != 1) return H3_ERR_BAD_LAYOUT;
+    }
+    if (!tensor_scale_ok(fmt, tx) || !tensor_scale_ok(fmt, tw)) return H3_ERR_UNSUPPORTED;
+    if (rows > 0x3fffffffLL || outs > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
+    p->M = (int)rows;
+    p->N = (int)outs;
+    p->ktiles = (int)((cols + BK - 1) / BK);
+    p->ksteps = (int)((cols + KSTEP - 1) / KSTEP);
+    p->chunks = (int)scale_chunks(fmt, cols);
+    p->sx = static_cast<const uint8_t *>(xs->data);
+    p->sw = static_cast<const uint8_t *>(ws->data);
+    p->y = static_cast<__nv_bfloat16 *>(y->data);
+    p->ldy = rows > 1 ? y->strides[0] : 0;
+    p->bias = bias && outs > 0 ? static_cast<const __nv_bfloat16 *>(bias->data) : nullptr;
+    p->t = tx * tw;
+    p->wide = aligned_to(y->data, 8) && p->ldy % 4 == 0;
+    return H3_OK;
+}
+
+}  // namespace fp4
+}  // namespace h3
+
+using namespace h3;
+
+extern "C" int h3_linear_fp4_quantized(const h3_tensor *y, const h3_tensor *x_codes, const h3_tensor *x_scales,
+                                       const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias,
+                                       int64_t cols, int32_t format, float x_tensor_scale, float w_tensor_scale,
+                                       void *stream) {
+    if (!x_codes) return H3_ERR_NULL;
+    fp4::Params p{};
+    H3_CHECK(fp4::check_product(y, x_codes, x_scales, w_codes, w_scales, bias, x_codes->shape[0], cols, format,
+                                x_tensor_scale, w_tensor_scale, &p));
+    if (p.M == 0 || p.N == 0) return H3_OK;
+    return format == fp4::MX ? fp4::multiply<fp4::MX>(x_codes, w_codes, p, (cudaStream_t)stream)
+                             : fp4::multiply<fp4::NV>(x_codes, w_codes, p, (cudaStream_t)stream);
+}
+
+extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *x_codes,
+                             const h3_tensor *x_scales, const h3_tensor *w_codes, const h3_tensor *w_scales,
+                             const h3_tensor *bias, int32_t format, float x_tensor_scale, float w_tensor_scale,
+                             void *stream) {
+    H3_CHECK(check_bf16(x));
+    if (x->ndim != 2) return H3_ERR_BAD_SHAPE;
+    fp4::Params p{};
+    H3_CHECK(fp4::check_product(y, x_codes, x_scales, w_codes, w_scales, bias, x->shape[0], x->shape[1], format,
+                                x_tensor_scale, w_tensor_scale, &p));
+    if (p.M == 0 || p.N == 0) return H3_OK;
+    H3_CHECK(fp4::quantize(x_codes, x_scales, x, format, x_tensor_scale, (cudaStream_t)stream));
+    p.dependent = 1;
+    return format == fp4::MX ? fp4::multiply<fp4::MX>(x_codes, w_codes, p, (cudaStream_t)stream)
+                             : fp4::multiply<fp4::NV>(x_codes, w_codes, p, (cudaStream_t)stream);
+}
+
+// device error word of this translation unit (bounded waits of the products)
+extern "C" unsigned int h3_fp4_device_error_read_and_clear(void) {
+    unsigned int v = 0, zero = 0;
+    cudaMemcpyFromSymbol(&v, h3::g_h3_device_error, sizeof(v));
+    cudaMemcpyToSymbol(h3::g_h3_device_error, &zero, sizeof(zero));
+    return v;
+}

@@ -1,0 +1,235 @@
+// Microscaled 4-bit quantisation of BF16 rows and its inverse (layout: fp4_common.cuh).
+//
+//   mxfp4  e = clamp(floor(log2 amax) - 2, -127, 127), scale 2^e   (block of 32)
+//   nvfp4  s = e4m3(amax / (6 t)), scale s t                       (block of 16)
+//   code   = e2m1 nearest-even of x / scale, at most 6 in magnitude
+// A block that holds an infinity or a NaN gets the NaN scale, so what is wrong stays
+// visible; a block whose scale rounds to zero gets zero codes.
+//
+// Every element is read once and written once: HBM-bound, 2 B in and 0.5 B + 1/block out
+// per element.  A thread owns 16 consecutive columns of a row (two 16-byte loads, one
+// 8-byte store of codes); an nvfp4 block is one thread's, an mxfp4 block two neighbours'.
+// The four scales of a chunk word are gathered by shuffle and stored as one word.
+#include <math.h>
+#include <string.h>
+
+#include "fp4_common.cuh"
+#include "h3_common.cuh"
+
+namespace h3 {
+namespace fp4 {
+
+constexpr int UNIT = 16;                 // columns per thread
+constexpr int THREADS = 256;
+
+struct Shape {
+    int64_t rows;
+    int cols, units;                     // units: 16-column pieces of a row, whole chunks
+    int code_units;                      // 16-column pieces of the code pitch
+    int log_tx;                          // threads along a row (power of two)
+    int chunks;                          // scale chunks along a row
+    int64_t ldx, ldc;                    // row strides: x in elements, codes in bytes
+    float tensor_scale;
+};
+
+// 16 columns of a row as packed BF16 pairs, zeros past the end
+template <bool VEC>
+__device__ __forceinline__ void load_unit(const __nv_bfloat16 *row, int col, int cols, uint32_t (&w)[8]) {
+    if (VEC && col + UNIT <= cols) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + col));
+        const uint4 b = __ldg(reinterpret_cast<const uint4 *>(row + col) + 1);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    } else {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t lo = col + 2 * i < cols ? __ldg(p + col + 2 * i) : 0;
+            const uint32_t hi = col + 2 * i + 1 < cols ? __ldg(p + col + 2 * i + 1) : 0;
+            w[i] = lo | (hi << 16);
+        }
+    }
+}
+
+// two e2m1 codes: `lo` in the low nibble
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
+        : "=r"(r)
+        : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3(float v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+    return r & 0xffu;
+}
+__device__ __forceinline__ float from_e4m3(uint32_t b) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)b));
+    return __half2float(__ushort_as_half((unsigned short)(h & 0xffff)));
+}
+
+template <int FMT, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+    quantize_kernel(const __nv_bfloat16 *x, uint8_t *codes, uint8_t *scales, Shape s) {
+    asm volatile("griddepcontrol.launch_dependents;");   // a product waiting on this may set itself up
+    const int tx = 1 << s.log_tx;
+    const int unit = (int)blockIdx.y * tx + (int)(threadIdx.x & (tx - 1));
+    const int64_t row = (int64_t)blockIdx.x * (THREADS >> s.log_tx) + (threadIdx.x >> s.log_tx);
+    const bool live = row < s.rows && unit < s.units;
+    uint32_t w[8] = {};
+    if (live) load_unit<VEC>(x + row * s.ldx, unit * UNIT, s.cols, w);
+
+    // magnitudes order as integers; at 0x7f80 and above they are infinite or NaN
+    uint32_t top2 = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top2 = __vmaxu2(top2, w[i] & 0x7fff7fffu);
+    uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+    if (FMT == MX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const bool bad = top >= 0x7f80u;
+
+    uint32_t byte, c[2] = {0, 0};
+    if (FMT == MX) {
+        // the exponent field of amax is floor(log2 amax) + 127 (0 below the normals)
+        const int e = (int)(top >> 7) - 2;
+        byte = bad ? 255u : (uint32_t)max(e, 0);
+        const float inv = __uint_as_float((254u - byte) << 23);      // 2^(127 - byte), exact
+        if (!bad) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i >> 2] |= e2m1x2(blo(w[i]) * inv, bhi(w[i]) * inv) << (8 * (i & 3));
+        }
+    } else {
+        const float amax = __uint_as_float(top << 16);
+        byte = bad ? 127u : e4m3(__fdiv_rn(amax, 6.0f * s.tensor_scale));
+        if (!bad && byte != 0) {
+            // x / scale lies on a border between two codes, a multiple of 1/4, or (x has 8
+            // significant bits, the scale 4) at least 1/300 of it away.  Adding and taking
+            // away 1.5 * 2^11 rounds the product with the reciprocal to a multiple of 2^-12,
+            // which puts the first kind exactly on its border and moves none across.
+            const float r = __frcp_rn(from_e4m3(byte) * s.tensor_scale);
+            constexpr float SNAP = 1.5f * 2048.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                c[i >> 2] |= e2m1x2(__fadd_rn(__fmaf_rn(blo(w[i]), r, SNAP), -SNAP),
+                                    __fadd_rn(__fmaf_rn(bhi(w[i]), r, SNAP), -SNAP))
+                             << (8 * (i & 3));
+        }
+    }
+    if (live && unit < s.code_units)
+        *reinterpret_cast<uint2 *>(codes + row * s.ldc + unit * (UNIT / 2)) = make_uint2(c[0], c[1]);
+
+    // the four scales of a chunk's word sit in 4 (nvfp4) or 8 (mxfp4, each twice) lanes
+    constexpr int STEP = FMT == MX ? 2 : 1;
+    uint32_t word = byte | (__shfl_down_sync(0xffffffffu, byte, STEP) << 8);
+    word |= __shfl_down_sync(0xffffffffu, word, 2 * STEP) << 16;
+    if (live && unit % (4 * STEP) == 0) {
+        const int64_t chunk = (row >> 7) * s.chunks + unit / (4 * STEP);
+        *reinterpret_cast<uint32_t *>(scales + chunk * CHUNK + (row & 31) * 16 + ((row >> 5) & 3) * 4) = word;
+    }
+}
+
+template <int FMT, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+    dequantize_kernel(__nv_bfloat16 *y, const uint8_t *codes, const uint8_t *scales, Shape s) {
+    const int tx = 1 << s.log_tx;
+    const int unit = (int)blockIdx.y * tx + (int)(threadIdx.x & (tx - 1));
+    const int64_t row = (int64_t)blockIdx.x * (THREADS >> s.log_tx) + (threadIdx.x >> s.log_tx);
+    const int col = unit * UNIT;
+    if (row >= s.rows || col >= s.cols) return;
+    const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes + row * s.ldc + unit * (UNIT / 2)));
+    const int block = FMT == MX ? unit >> 1 : unit;
+    const uint32_t byte = __ldg(scales + ((row >> 7) * s.chunks + (block >> 2)) * CHUNK + (row & 31) * 16 +
+                                ((row >> 5) & 3) * 4 + (block & 3));
+    float scale;
+    if (FMT == MX) scale = byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte == 0 ? 1u << 22 : byte << 23);
+    else scale = from_e4m3(byte) * s.tensor_scale;      // cvt makes byte 127 a NaN
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xffu;
+        uint32_t h;
+        asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
+        const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&h));
+        // 2 significant bits times 4: exact in BF16
+        w[i] = bf2u(__floats2bfloat162_rn(f.x * scale, f.y * scale));
+    }
+    __nv_bfloat16 *dst = y + row * s.ldx + col;
+    if (VEC && col + UNIT <= s.cols) {
+        reinterpret_cast<uint4 *>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+        uint16_t *p = reinterpret_cast<uint16_t *>(dst);
+#pragma unroll
+        for (int i = 0; i < UNIT; ++i)
+            if (col + i < s.cols) p[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
+}
+
+// Shared checks and launch shape; `x` is the BF16 side.
+int plan(const h3_tensor *x, const h3_tensor *codes, const h3_tensor *scales, int fmt, float tensor_scale, Shape *s,
+         dim3 *grid, bool *vec) {
+    H3_CHECK(check_bf16(x));
+    if (x->ndim != 2 || x->shape[1] < 1) return H3_ERR_BAD_SHAPE;
+    H3_CHECK(check_held(codes, scales, fmt, x->shape[0], x->shape[1]));
+    if (!tensor_scale_ok(fmt, tensor_scale)) return H3_ERR_UNSUPPORTED;
+    if (x->shape[0] > 0x7fffffffLL || x->shape[1] > (1 << 24)) return H3_ERR_UNSUPPORTED;
+    if (x->shape[0] == 0) return H3_OK;
+    if ((x->shape[1] > 1 && x->strides[1] != 1) || (x->shape[0] > 1 && x->strides[0] < 0)) return H3_ERR_BAD_LAYOUT;
+    s->rows = x->shape[0];
+    s->cols = (int)x->shape[1];
+    s->chunks = (int)scales->shape[1];
+    s->units = s->chunks * (fmt == MX ? 8 : 4);
+    s->code_units = (int)codes->shape[1] / (UNIT / 2);
+    s->ldx = x->shape[0] > 1 ? x->strides[0] : 0;
+    s->ldc = x->shape[0] > 1 ? codes->strides[0] : 0;
+    s->tensor_scale = tensor_scale;
+    // threads along a row: enough for short rows, at most 64 so that long rows waste few
+    s->log_tx = 3;
+    while (s->log_tx < 6 && (1 << s->log_tx) < s->units) ++s->log_tx;
+    const int ty = THREADS >> s->log_tx;
+    *grid = dim3((unsigned)((s->rows + ty - 1) / ty), (unsigned)((s->units + (1 << s->log_tx) - 1) >> s->log_tx));
+    *vec = aligned16(x->data) && s->ldx % 8 == 0;
+    return H3_OK;
+}
+
+int quantize(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int fmt, float tensor_scale,
+             cudaStream_t stream) {
+    Shape s{};
+    dim3 grid;
+    bool vec;
+    H3_CHECK(plan(x, codes, scales, fmt, tensor_scale, &s, &grid, &vec));
+    if (x->shape[0] == 0) return H3_OK;
+    auto kernel = fmt == MX ? (vec ? quantize_kernel<MX, true> : quantize_kernel<MX, false>)
+                            : (vec ? quantize_kernel<NV, true> : quantize_kernel<NV, false>);
+    kernel<<<grid, THREADS, 0, stream>>>(static_cast<const __nv_bfloat16 *>(x->data),
+                                         static_cast<uint8_t *>(codes->data), static_cast<uint8_t *>(scales->data), s);
+    return launch_status();
+}
+
+}  // namespace fp4
+}  // namespace h3
+
+using namespace h3;
+
+extern "C" int h3_quantize_fp4(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int32_t format,
+                               float tensor_scale, void *stream) {
+    return fp4::quantize(codes, scales, x, format, tensor_scale, (cudaStream_t)stream);
+}
+
+extern "C" int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tensor *scales, int32_t format,
+                                 float tensor_scale, void *stream) {
+    fp4::Shape s{};
+    dim3 grid;
+    bool vec;
+    H3_CHECK(fp4::plan(y, codes, scales, format, tensor_scale, &s, &grid, &vec));
+    if (y->shape[0] == 0) return H3_OK;
+    if (y->shape[0] > 1 && y->strides[0] < y->shape[1]) return H3_ERR_BAD_LAYOUT;   // rows would overlap
+    auto kernel = format == fp4::MX ? (vec ? fp4::dequantize_kernel<fp4::MX, true> : fp4::dequantize_kernel<fp4::MX, false>)
+                                    : (vec ? fp4::dequantize_kernel<fp4::NV, true> : fp4::dequantize_kernel<fp4::NV, false>);
+    kernel<<<grid, fp4::THREADS, 0, (cudaStream_t)stream>>>(static_cast<__nv_bfloat16 *>(y->data),
+                                                            static_cast<const uint8_t *>(codes->data),
+                                                            static_cast<const uint8_t *>(scales->data), s);
+    return launch_status();
+}

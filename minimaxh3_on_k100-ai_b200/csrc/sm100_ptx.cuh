@@ -180,6 +180,13 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(cluster_bar)
         : "memory");
 }
+// `bytes` (a multiple of 16) contiguous bytes, both addresses 16-byte aligned
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
 // Bring a box of the tensor into L2 ahead of its tma_load_4d (no shared-memory write, no barrier).
 __device__ __forceinline__ void tma_prefetch_l2_4d(const CUtensorMap *map, int c0, int c1, int c2, int c3) {
     asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
@@ -280,6 +287,39 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar) {
                  : "memory");
 }
 
+// Block-scaled 4-bit forms: A and B hold e2m1 codes two a byte, K-major, 64 K elements
+// (32 bytes) per instruction; the scales sit in tensor memory, row r%32 + 32j of the
+// operand in lane r%32, column j, one byte per block.  MXF4: blocks of 32, power-of-two
+// scales, two of a column's four bytes per instruction (which two: the descriptor's
+// scale ids); otherwise blocks of 16, e4m3 scales, all four bytes.
+template <bool MXF4, bool PAIR>
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+#define H3_UMMA_FP4(GROUP, KIND)                                                                             \
+    asm volatile("{\n\t.reg .pred p;\n\t"                                                                    \
+                 "setp.ne.b32 p, %6, 0;\n\t"                                                                 \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"( \
+                     d_tmem),                                                                                \
+                 "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)         \
+                 : "memory")
+    if (MXF4) {
+        if (PAIR) H3_UMMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+        else H3_UMMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+    } else {
+        if (PAIR) H3_UMMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+        else H3_UMMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    }
+#undef H3_UMMA_FP4
+}
+// 512 bytes of shared memory (32 rows of 16 bytes) to 4 columns of tensor memory, the
+// same 32 lanes repeated in all four quarters; PAIR: in both CTAs of the pair, each from
+// its own shared memory.  Ordered before this thread's later MMAs of the same group.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t d_tmem, uint64_t s_desc) {
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread t gets row (lane base + t), columns [col, col+32)
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
@@ -290,6 +330,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// the same for 16 columns
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -321,6 +370,21 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
     d |= 1ull << 46;
     d |= 2ull << 61;
     return d;
+}
+
+// Shared-memory descriptor of rows of 16 bytes without swizzle, 8-row groups 128 bytes
+// apart (layout 0): the scale chunks tcgen05.cp reads.
+__device__ __forceinline__ uint64_t smem_desc_rows16(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) |
+           (1ull << 46);
+}
+
+// Instruction descriptor, kind::mxf4 / kind::mxf4nvf4, e2m1 x e2m1 -> F32, K = 64.
+//   [4,6) B scale id | [7,10) A fmt 1=E2M1 | [10,12) B fmt 1=E2M1 | [17,23) N>>3 |
+//   bit 23 scale type (0=UE4M3, 1=UE8M0) | [27,29) M>>7 | [29,31) A scale id
+__host__ __device__ constexpr uint32_t idesc_fp4(int M, int N, bool ue8m0, uint32_t sf_id) {
+    return (sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
+           ((uint32_t)(M >> 7) << 27) | (sf_id << 29);
 }
 
 // Instruction descriptor, kind::f16, BF16 x BF16 -> F32.

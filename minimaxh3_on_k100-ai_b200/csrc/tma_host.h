@@ -42,4 +42,19 @@ inline int make_tmap_bf16(CUtensorMap *map, void *base, int rank, const cuuint64
     return r == CUDA_SUCCESS ? H3_OK : H3_ERR_BAD_LAYOUT;
 }
 
+// The same for a matrix of bytes [rows, width] with rows `pitch` bytes apart.
+inline int make_tmap_bytes(CUtensorMap *map, void *base, uint64_t width, uint64_t rows, uint64_t pitch,
+                           uint32_t box_width, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return H3_ERR_DRIVER;
+    const cuuint64_t dims[2] = {width, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_width, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? H3_OK : H3_ERR_BAD_LAYOUT;
+}
+
 }  // namespace h3

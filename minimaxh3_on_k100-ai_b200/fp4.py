@@ -1,0 +1,215 @@
+"""Microscaled 4-bit matrices and projections on the sm_100a C-ABI library.
+
+A block of consecutive columns of a row shares one scale; a value is an e2m1 code
+(0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times that scale:
+
+* ``"mxfp4"``: blocks of 32, the scale a power of two;
+* ``"nvfp4"``: blocks of 16, the scale an e4m3 number times ``tensor_scale``, one power
+  of two for the whole matrix (``fp4_tensor_scale`` gives one that fits).
+
+Weights are held as ``Fp4Tensor`` (made once, by ``quantize_fp4`` from BF16 or by
+``pack_fp4`` from a checkpoint's codes and scales); ``linear_fp4`` quantises its
+activations on the way in.  Inference only: nothing here takes part in autograd.
+No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import call, desc, require_cuda, stream_of
+
+__all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_fp4", "quantize_fp4_", "dequantize_fp4",
+           "dequantize_fp4_", "pack_fp4", "unpack_fp4", "linear_fp4", "linear_fp4_"]
+
+FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_FORMAT = {"mxfp4": 0, "nvfp4": 1}
+
+
+def _check_format(fmt: str) -> int:
+    try:
+        return _FORMAT[fmt]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown 4-bit format {fmt!r}: 'mxfp4' or 'nvfp4'") from None
+
+
+def _check_tensor_scale(fmt: str, scale: float) -> float:
+    scale = float(scale)
+    if fmt == "mxfp4":
+        if scale != 1.0:
+            raise ValueError("mxfp4 has no tensor scale")
+    elif not (2.0 ** -64 <= scale <= 2.0 ** 64) or math.frexp(scale)[0] != 0.5:
+        raise ValueError(f"the tensor scale must be a power of two in [2^-64, 2^64], got {scale}")
+    return scale
+
+
+@dataclass
+class Fp4Tensor:
+    """A matrix of ``rows`` x ``cols`` 4-bit values: ``codes`` uint8
+    [rows, ceil(cols/32)*16] (two codes a byte) and ``scales`` uint8
+    [ceil(rows/128), ceil(blocks/4), 512], as the products read them."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    cols: int
+    format: str
+    tensor_scale: float = 1.0
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def fp4_empty(rows: int, cols: int, format: str = "nvfp4", tensor_scale: float = 1.0, device="cuda") -> Fp4Tensor:
+    """An uninitialised 4-bit matrix (a workspace, or the target of ``quantize_fp4_``)."""
+    _check_format(format)
+    if rows < 0 or cols < 1:
+        raise ValueError(f"a 4-bit matrix has at least one column, got [{rows}, {cols}]")
+    per_chunk = 4 * FP4_BLOCK[format]
+    codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=device)
+    scales = torch.empty(((rows + 127) // 128, (cols + per_chunk - 1) // per_chunk, 512), dtype=torch.uint8,
+                         device=device)
+    return Fp4Tensor(codes, scales, rows, cols, format, _check_tensor_scale(format, tensor_scale))
+
+
+def fp4_tensor_scale(amax: float) -> float:
+    """The smallest power of two t with amax <= 6 * 448 * t: the finest nvfp4 tensor scale
+    at which no block of a matrix with entries up to ``amax`` saturates."""
+    amax = float(amax)
+    if not math.isfinite(amax) or amax < 0:
+        raise ValueError(f"amax must be finite and not negative, got {amax}")
+    if amax == 0:
+        return 1.0
+    m, e = math.frexp(amax / 2688.0)        # m in [0.5, 1)
+    return 2.0 ** max(-64, min(64, e - 1 if m == 0.5 else e))
+
+
+def _rows_of(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+def _rows_to_write(out: torch.Tensor) -> torch.Tensor:
+    try:
+        return out if out.dim() == 2 else out.view(-1, out.shape[-1])
+    except RuntimeError:
+        raise ValueError("out's leading dimensions must collapse to rows without a copy") from None
+
+
+# ---------------------------------------------------------------------------
+# quantisation
+# ---------------------------------------------------------------------------
+def quantize_fp4_(out: Fp4Tensor, x: torch.Tensor) -> Fp4Tensor:
+    """Quantise x [..., cols] BF16 into ``out`` (its format and tensor scale)."""
+    require_cuda(out.codes, out.scales, x)
+    x2 = _rows_of(x)
+    if x2.shape != (out.rows, out.cols):
+        raise ValueError(f"x has shape {tuple(x2.shape)}, the 4-bit matrix {out.shape}")
+    call("h3_quantize_fp4", desc(out.codes), desc(out.scales), desc(x2), _FORMAT[out.format], out.tensor_scale,
+         stream_of(x))
+    return out
+
+
+def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: float = 1.0) -> Fp4Tensor:
+    """x [..., cols] BF16 as a 4-bit matrix of its rows."""
+    x2 = _rows_of(x)
+    return quantize_fp4_(fp4_empty(x2.shape[0], x2.shape[1], format, tensor_scale, x.device), x2)
+
+
+def dequantize_fp4_(out: torch.Tensor, q: Fp4Tensor) -> torch.Tensor:
+    require_cuda(out, q.codes, q.scales)
+    if tuple(out.shape) != q.shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, the 4-bit matrix {q.shape}")
+    call("h3_dequantize_fp4", desc(out), desc(q.codes), desc(q.scales), _FORMAT[q.format], q.tensor_scale,
+         stream_of(out))
+    return out
+
+
+def dequantize_fp4(q: Fp4Tensor) -> torch.Tensor:
+    """The values a 4-bit matrix stands for, [rows, cols] BF16 (exact)."""
+    return dequantize_fp4_(torch.empty(q.rows, q.cols, dtype=torch.bfloat16, device=q.device), q)
+
+
+def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, format: str, cols: int | None = None,
+             tensor_scale: float = 1.0) -> Fp4Tensor:
+    """A 4-bit matrix from row-major parts, as checkpoints store them: ``codes`` uint8
+    [rows, ceil(cols/2)] (column 2i in the low nibble of byte i) and ``scales`` uint8 (or
+    e4m3) [rows, ceil(cols/block)].  A set-up step: lays the scales out once, in torch."""
+    _check_format(format)
+    if scales.dtype != torch.uint8 and scales.element_size() == 1:
+        scales = scales.view(torch.uint8)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("codes and scales must be bytes")
+    if codes.dim() != 2 or scales.dim() != 2 or codes.shape[0] != scales.shape[0]:
+        raise ValueError("codes and scales are matrices of the same rows")
+    if codes.device != scales.device:
+        raise ValueError("codes and scales must be on the same device")
+    rows = codes.shape[0]
+    cols = 2 * codes.shape[1] if cols is None else int(cols)
+    block = FP4_BLOCK[format]
+    blocks = (cols + block - 1) // block
+    if cols < 1 or codes.shape[1] != (cols + 1) // 2 or scales.shape[1] != blocks:
+        raise ValueError(f"{cols} columns need {(cols + 1) // 2} code bytes and {blocks} scales a row, got "
+                         f"{codes.shape[1]} and {scales.shape[1]}")
+    out = fp4_empty(rows, cols, format, tensor_scale, codes.device)
+    out.codes.zero_()
+    out.codes[:, : codes.shape[1]] = codes
+    if cols % 2:
+        out.codes[:, cols // 2] &= 0x0F
+    chunks_m, chunks_k = out.scales.shape[:2]
+    padded = torch.zeros(chunks_m * 128, chunks_k * 4, dtype=torch.uint8, device=codes.device)
+    padded[:rows, :blocks] = scales
+    # row 128 a + 32 j + i, block 4 c + b -> chunk [a][c], byte 16 i + 4 j + b
+    out.scales.copy_(padded.view(chunks_m, 4, 32, chunks_k, 4).permute(0, 3, 2, 1, 4).reshape(out.scales.shape))
+    return out
+
+
+def unpack_fp4(q: Fp4Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``pack_fp4``'s parts back: codes [rows, ceil(cols/2)] and scales [rows, ceil(cols/block)]."""
+    blocks = (q.cols + FP4_BLOCK[q.format] - 1) // FP4_BLOCK[q.format]
+    a, c = q.scales.shape[:2]
+    scales = q.scales.view(a, c, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(a * 128, c * 4)
+    return q.codes[:, : (q.cols + 1) // 2].clone(), scales[: q.rows, :blocks].contiguous()
+
+
+# ---------------------------------------------------------------------------
+# projection
+# ---------------------------------------------------------------------------
+def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
+                x_tensor_scale: float = 1.0) -> torch.Tensor:
+    """out [..., N] BF16 = x W^T (+ bias), both in ``weight``'s 4-bit format, fp32
+    accumulation, one rounding.  ``x`` BF16 [..., K] is quantised on the way in (with
+    ``x_tensor_scale`` for nvfp4), or given as an ``Fp4Tensor`` (then out is [M, N]) when
+    several projections share it."""
+    o2 = _rows_to_write(out)
+    if isinstance(x, Fp4Tensor):
+        require_cuda(out, x.codes, x.scales, weight.codes, weight.scales, bias)
+        if x.format != weight.format:
+            raise ValueError(f"x is {x.format}, the weight {weight.format}")
+        if x.cols != weight.cols:
+            raise ValueError(f"x has {x.cols} columns, the weight {weight.cols}")
+        call("h3_linear_fp4_quantized", desc(o2), desc(x.codes), desc(x.scales), desc(weight.codes),
+             desc(weight.scales), desc(bias), x.cols, _FORMAT[weight.format], x.tensor_scale, weight.tensor_scale,
+             stream_of(out))
+        return out
+    x2 = _rows_of(x)
+    if x2.shape[1] != weight.cols:
+        raise ValueError(f"x has {x2.shape[1]} columns, the weight {weight.cols}")
+    require_cuda(out, x, weight.codes, weight.scales, bias)
+    work = fp4_empty(x2.shape[0], weight.cols, weight.format, x_tensor_scale, x.device)
+    call("h3_linear_fp4", desc(o2), desc(x2), desc(work.codes), desc(work.scales), desc(weight.codes),
+         desc(weight.scales), desc(bias), _FORMAT[weight.format], work.tensor_scale, weight.tensor_scale,
+         stream_of(x))
+    return out
+
+
+def linear_fp4(x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
+               x_tensor_scale: float = 1.0) -> torch.Tensor:
+    lead = (x.rows,) if isinstance(x, Fp4Tensor) else x.shape[:-1]
+    out = torch.empty(*lead, weight.rows, dtype=torch.bfloat16, device=x.device)
+    return linear_fp4_(out, x, weight, bias, x_tensor_scale)
