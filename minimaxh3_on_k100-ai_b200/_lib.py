@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -113,22 +114,29 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+# H3Tensor's bytes for 0..4 dimensions: one pack and one copy cost a third of what
+# setting the fields one by one does, and a small launch is mostly host time
+_PACK = [struct.Struct(f"P{n}q{(4 - n) * 8}x{n}q{(4 - n) * 8}xii").pack for n in range(5)]
+
+
 def desc(t: torch.Tensor | None) -> H3Tensor | None:
     if t is None:
         return None
-    if t.dim() > 4:
-        raise ValueError(f"at most 4 dims supported, got {t.dim()}")
-    d = H3Tensor()
-    d.data = t.data_ptr()
-    for i in range(t.dim()):
-        d.shape[i] = t.shape[i]
-        d.strides[i] = t.stride(i)
-    d.ndim = t.dim()
-    try:
-        d.dtype = _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"unsupported dtype {t.dtype}") from None
-    return d
+    n = t.dim()
+    if n > 4:
+        raise ValueError(f"at most 4 dims supported, got {n}")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {t.dtype}")
+    return H3Tensor.from_buffer_copy(_PACK[n](t.data_ptr(), *t.shape, *t.stride(), n, code))
+
+
+def desc_rows(ptr: int, dtype: torch.dtype, *shape: int) -> H3Tensor:
+    """The descriptor of a contiguous tensor at ``ptr`` (a piece of a workspace)."""
+    strides = [1] * len(shape)
+    for i in range(len(shape) - 1, 0, -1):
+        strides[i - 1] = strides[i] * shape[i]
+    return H3Tensor.from_buffer_copy(_PACK[len(shape)](ptr, *shape, *strides, len(shape), _DTYPES[dtype]))
 
 
 def ref(d: H3Tensor | None):
@@ -136,7 +144,7 @@ def ref(d: H3Tensor | None):
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def check(status: int, op: str) -> None:
@@ -154,10 +162,10 @@ CALLS = {"n": 0}
 
 
 def call(name: str, *args) -> None:
-    lib = load()
-    conv = [ctypes.byref(a) if isinstance(a, H3Tensor) else a for a in args]
     CALLS["n"] += 1
-    check(getattr(lib, name)(*conv), name)
+    status = getattr(_lib or load(), name)(*args)   # ctypes passes an H3Tensor by reference
+    if status:
+        check(status, name)
 
 
 def check_device(where: str) -> None:
@@ -170,18 +178,18 @@ def check_device(where: str) -> None:
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:
-    dev = None
+    dev = -1
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError("H3 ops take CUDA tensors only (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if dev < 0:
+            dev = t.get_device()
+        elif t.get_device() != dev:
             raise ValueError("all tensors must be on the same device")
-    if dev is not None and dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev} but the current device is cuda:{torch.cuda.current_device()}; "
+    if dev >= 0 and dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{dev} but the current device is cuda:{torch.cuda.current_device()}; "
                          "call under torch.cuda.device(...)")
 
 

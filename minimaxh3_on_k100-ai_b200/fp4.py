@@ -19,7 +19,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import call, desc, require_cuda, stream_of
+from ._lib import call, desc, desc_rows, require_cuda, stream_of
 
 __all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_fp4", "quantize_fp4_", "dequantize_fp4",
            "dequantize_fp4_", "pack_fp4", "unpack_fp4", "linear_fp4", "linear_fp4_"]
@@ -37,10 +37,11 @@ def _check_format(fmt: str) -> int:
 
 def _check_tensor_scale(fmt: str, scale: float) -> float:
     scale = float(scale)
+    if scale == 1.0:
+        return scale
     if fmt == "mxfp4":
-        if scale != 1.0:
-            raise ValueError("mxfp4 has no tensor scale")
-    elif not (2.0 ** -64 <= scale <= 2.0 ** 64) or math.frexp(scale)[0] != 0.5:
+        raise ValueError("mxfp4 has no tensor scale")
+    if not (2.0 ** -64 <= scale <= 2.0 ** 64) or math.frexp(scale)[0] != 0.5:
         raise ValueError(f"the tensor scale must be a power of two in [2^-64, 2^64], got {scale}")
     return scale
 
@@ -201,15 +202,20 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
     if x2.shape[1] != weight.cols:
         raise ValueError(f"x has {x2.shape[1]} columns, the weight {weight.cols}")
     require_cuda(out, x, weight.codes, weight.scales, bias)
-    work = fp4_empty(x2.shape[0], weight.cols, weight.format, x_tensor_scale, x.device)
-    call("h3_linear_fp4", desc(o2), desc(x2), desc(work.codes), desc(work.scales), desc(weight.codes),
-         desc(weight.scales), desc(bias), _FORMAT[weight.format], work.tensor_scale, weight.tensor_scale,
-         stream_of(x))
+    scale = _check_tensor_scale(weight.format, x_tensor_scale)
+    # x in 4 bits, codes then scales, in one allocation
+    rows, pitch = x2.shape[0], (weight.cols + 31) // 32 * 16
+    chunks_m, chunks_k = (rows + 127) // 128, weight.scales.shape[1]
+    work = torch.empty(rows * pitch + chunks_m * chunks_k * 512, dtype=torch.uint8, device=x.device)
+    at = work.data_ptr()
+    call("h3_linear_fp4", desc(o2), desc(x2), desc_rows(at, torch.uint8, rows, pitch),
+         desc_rows(at + rows * pitch, torch.uint8, chunks_m, chunks_k, 512), desc(weight.codes), desc(weight.scales),
+         desc(bias), _FORMAT[weight.format], scale, weight.tensor_scale, stream_of(x))
     return out
 
 
 def linear_fp4(x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
                x_tensor_scale: float = 1.0) -> torch.Tensor:
     lead = (x.rows,) if isinstance(x, Fp4Tensor) else x.shape[:-1]
-    out = torch.empty(*lead, weight.rows, dtype=torch.bfloat16, device=x.device)
+    out = torch.empty((*lead, weight.rows), dtype=torch.bfloat16, device=x.device)
     return linear_fp4_(out, x, weight, bias, x_tensor_scale)
