@@ -326,6 +326,12 @@ int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *x_cod
                   const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int32_t format,
                   float x_tensor_scale, float w_tensor_scale, void *stream);
 
+/* Form of the 4-bit projections: 0 = chosen per launch, 1 = weight rows as the M side and
+ * K split over a cluster (few rows of x), 2 = CTA-pair 256 x 256 tiles.  The forms add in
+ * different orders, so their results can differ in the last bit.  Returns the previous
+ * setting, or -1 for a value outside 0..2 (setting unchanged).  A tuning and test hook. */
+int h3_fp4_variant(int variant);
+
 /* h3_linear_fp4 for x that is in 4 bits already (several projections of the same rows);
  * cols = K. */
 int h3_linear_fp4_quantized(const h3_tensor *y, const h3_tensor *x_codes, const h3_tensor *x_scales,

@@ -79,6 +79,7 @@ SIGNATURES = {
     "h3_linear_qkv_norm_rope": [P, P, P, P, P, _I, P, P, P, P, _F, _V],
     "h3_quantize_fp4": [P, P, P, _I, _F, _V],
     "h3_dequantize_fp4": [P, P, P, _I, _F, _V],
+    "h3_fp4_variant": [ctypes.c_int],
     "h3_linear_fp4": [P, P, P, P, P, P, P, _I, _F, _F, _V],
     "h3_linear_fp4_quantized": [P, P, P, P, P, P, ctypes.c_int64, _I, _F, _F, _V],
     "h3_linear_f32": [P, P, P, P, _V],

@@ -11,6 +11,14 @@
 // cluster of up to 8 CTAs splits K, each CTA leaves its fp32 tile in shared memory and
 // sums its share of the columns over the cluster in rank order (fixed order, no atomics,
 // no scratch in global memory).  Bound by reading the weights (HBM).
+//
+// tile form: persistent CTA pairs (cta_group::2), 256 x 256 output tiles, K in tiles of 256
+// (one 128-byte swizzle span of codes) through a 5-slot TMA ring.  Each CTA loads its 128 x
+// rows, half the tile's w rows, and the scales of its x rows and of all the w rows; the
+// leader copies both CTAs' scales to tensor memory and issues the MMAs.  Two accumulators
+// of 256 columns and the scales do not fit the 512 columns, so the accumulators share 96:
+// the epilogue reads those first and then lets the next tile start, so all but that read
+// overlaps the next tile's products.
 #include <math.h>
 #include <stdint.h>
 #include <string.h>
@@ -183,9 +191,10 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     tc_fence_after();
     // lane = weight row: column c of the tile becomes 128 consecutive floats
     const uint32_t red = smem_u32(smem);
+    const int cols = min(BN, p.M - m0);
     if (ok) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < BN; c0 += 16) {
+        for (int c0 = 0; c0 < cols; c0 += 16) {
             uint32_t v[16];
             if (nk > 0) {
                 tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + c0, v);
@@ -207,14 +216,16 @@ __global__ void __launch_bounds__(SWAP_THREADS)
             for (int e = 0; e < 4; ++e)
                 if (n + e < p.N) b[e] = __bfloat162float(p.bias[n + e]);
         }
-        const int cols = min(BN, p.M - m0);
         for (int c = rank * 4 + warp; c < cols; c += split * 4) {
-            float4 acc = ld_cluster_f4(red + (c * 128 + lane * 4) * 4, 0);
-#pragma unroll 1
-            for (int r = 1; r < split; ++r) {
-                const float4 o = ld_cluster_f4(red + (c * 128 + lane * 4) * 4, (uint32_t)r);
-                acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
-            }
+            // all ranks' pieces are requested before the first is needed
+            float4 part[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < split) part[r] = ld_cluster_f4(red + (c * 128 + lane * 4) * 4, (uint32_t)r);
+            float4 acc = part[0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r)
+                if (r < split) acc.x += part[r].x, acc.y += part[r].y, acc.z += part[r].z, acc.w += part[r].w;
             const float f[4] = {fmaf(acc.x, p.t, b[0]), fmaf(acc.y, p.t, b[1]), fmaf(acc.z, p.t, b[2]),
                                 fmaf(acc.w, p.t, b[3])};
             __nv_bfloat16 *dst = p.y + (int64_t)(m0 + c) * p.ldy + n;
@@ -245,36 +256,45 @@ int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_
                              xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, BN));
     H3_CHECK(make_tmap_bytes(&tw, wc->data, wc->shape[1], wc->shape[0],
                              wc->shape[0] > 1 ? wc->strides[0] : wc->shape[1], 128, 128));
-    static std::atomic<bool> ready[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
-    if (!ready[dev].load()) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-            return H3_ERR_LAUNCH;
-        ready[dev].store(true);
-    }
     p.num_m = (p.M + BN - 1) / BN;
     p.num_n = (p.N + 127) / 128;
     if (p.num_m > 65535 || p.num_n > 65535) return H3_ERR_UNSUPPORTED;
-    // K shares: as many as two CTAs per SM leave room for
-    const int64_t tiles = (int64_t)p.num_m * p.num_n, slots = 2 * num_sms();
-    int split = (int)(slots / tiles);
-    split = split < 1 ? 1 : split > 8 ? 8 : split;
-    if (split > p.ktiles) split = p.ktiles;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(split, p.num_n, p.num_m);
     cfg.blockDim = dim3(SWAP_THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
     cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // Per device: how many clusters of 1..8 CTAs are resident at once.  A cluster stays
+    // within one group of SMs, so 8-CTA clusters fill fewer SMs than their number suggests.
+    static std::atomic<int> resident[64][9];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
+    if (resident[dev][1].load() == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+            return H3_ERR_LAUNCH;
+        for (int c = 8; c >= 1; --c) {
+            attr[0].val.clusterDim.x = c;
+            cfg.gridDim = dim3(c, 1024, 1);
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return H3_ERR_LAUNCH;
+            resident[dev][c].store(n);
+        }
+    }
+    // K shares: as many as run in one wave
+    const int64_t tiles = (int64_t)p.num_m * p.num_n;
+    int split = p.ktiles < 8 ? p.ktiles : 8;
+    while (split > 1 && resident[dev][split].load() < tiles) --split;
+    attr[0].val.clusterDim.x = split;
+    cfg.gridDim = dim3(split, p.num_n, p.num_m);
     cfg.numAttrs = p.dependent ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, p) != cudaSuccess) {
         cudaGetLastError();
@@ -283,8 +303,311 @@ int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_
     return launch_status();
 }
 
+// ---------------------------------------------------------------------------
+// tile form: persistent CTA pairs, 256 x 256 output tiles
+// ---------------------------------------------------------------------------
+constexpr int TILE = 256;                        // rows and columns of a pair's output tile
+constexpr int TILE_THREADS = 256;
+constexpr int GROUP_N = 8;                       // column tiles per raster group
+
+template <int FMT>
+struct Pair {
+    static constexpr int CH = tile_chunks(FMT);
+    static constexpr int SF_BYTES = CH * CHUNK;               // scales of 128 rows per K tile
+    static constexpr int OFF_B = 128 * 128;                   // this CTA's 128 x rows, then half the tile's w rows
+    static constexpr int OFF_SFA = 2 * OFF_B;
+    static constexpr int OFF_SFB = OFF_SFA + SF_BYTES;        // all 256 w rows: each CTA multiplies with every one
+    static constexpr int STAGE = OFF_SFB + 2 * SF_BYTES;      // a multiple of 1024
+    static constexpr int STAGES = 5;
+    static constexpr int STORE_WARP = 32 * 64;                // an epilogue warp's 32 rows x 32 columns
+    static constexpr int OFF_STORE = STAGES * STAGE;
+    static constexpr int OFF_BAR = OFF_STORE + 4 * STORE_WARP;
+    static constexpr int SMEM = OFF_BAR + (2 * STAGES + 2) * 8 + 16 + 1024;
+    static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
+    // Tensor memory: two 256-column accumulators sharing 96 columns, and two buffers of
+    // scales (4 columns per 128 rows and chunk: 4 CH of x, 8 CH of w)
+    static constexpr int ACC1 = 160;
+    static constexpr int SF_COL0 = 416;
+    static constexpr int SF_COLS = 12 * CH;
+    static_assert(SF_COL0 + 2 * SF_COLS <= 512 && ACC1 + TILE <= SF_COL0, "tensor memory");
+};
+
+__device__ __forceinline__ void tile_at(const Params &p, int tile, int &m, int &n) {
+    const int span = GROUP_N * p.num_m;
+    const int g = tile / span, r = tile - g * span;
+    const int gw = min(GROUP_N, p.num_n - g * GROUP_N);
+    m = r / gw;
+    n = g * GROUP_N + (r - m * gw);
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+    tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
+                const __grid_constant__ CUtensorMap tsx, const __grid_constant__ CUtensorMap tsw, Params p) {
+    using C = Pair<FMT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
+    uint64_t *empty = full + C::STAGES;
+    uint64_t *acc_full = empty + C::STAGES;     // the tile's products have landed
+    uint64_t *acc_free = acc_full + 1;          // leader's: the columns both accumulators share have been read
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_free + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int first = (int)(blockIdx.x >> 1), step = (int)(gridDim.x >> 1);
+    const int num_tiles = p.num_m * p.num_n;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_free, 8);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        tma_prefetch_desc(&tx);
+        tma_prefetch_desc(&tw);
+        tma_prefetch_desc(&tsx);
+        tma_prefetch_desc(&tsw);
+        if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = first; tile < num_tiles && ok; tile += step) {
+            int m, n;
+            tile_at(p, tile, m, n);
+            for (int kt = 0; kt < p.ktiles; ++kt, ++it) {
+                const uint32_t slot = it % C::STAGES;
+                ok = mbar_wait(&empty[slot], ((it / C::STAGES) & 1) ^ 1, abort_flag);
+                if (!ok) break;
+                // both CTAs' bytes are counted on the leader's barrier
+                const uint32_t bar = mapa_shared(&full[slot], 0);
+                if (rank == 0) mbar_expect_tx(&full[slot], 2 * C::STAGE);
+                uint8_t *st = smem + slot * C::STAGE;
+                tma_load_2d_pair(st, &tx, bar, kt * 128, m * TILE + (int)rank * 128);
+                tma_load_2d_pair(st + C::OFF_B, &tw, bar, kt * 128, n * TILE + (int)rank * 128);
+                tma_load_2d_pair(st + C::OFF_SFA, &tsx, bar, kt * (C::SF_BYTES / 8), 2 * m + (int)rank);
+                tma_load_2d_pair(st + C::OFF_SFB, &tsw, bar, kt * (C::SF_BYTES / 8), 2 * n);
+            }
+        }
+        // the leader's last commits arrive here: none may land after this CTA has gone
+        for (uint32_t i = 0; i < C::STAGES && ok; ++i) {
+            if (it < i + 1) break;
+            const uint32_t u = it - 1 - i;
+            ok = mbar_wait(&empty[u % C::STAGES], (u / C::STAGES) & 1, abort_flag);
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        const uint32_t base = smem_u32(smem);
+        uint32_t it = 0, lt = 0;
+        bool ok = true;
+        for (int tile = first; tile < num_tiles && ok; tile += step, ++lt) {
+            // the accumulator two tiles back has been read wholly before the last one's shared columns
+            if (lt > 0) ok = mbar_wait_cluster(acc_free, (lt - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + ((lt & 1) ? C::ACC1 : 0);
+            for (int kt = 0; kt < p.ktiles; ++kt, ++it) {
+                const uint32_t slot = it % C::STAGES;
+                ok = mbar_wait(&full[slot], (it / C::STAGES) & 1, abort_flag);
+                // two scale buffers: the MMAs two K tiles back must have read this one
+                if (ok && it >= 2)
+                    ok = mbar_wait(&empty[(it - 2) % C::STAGES], ((it - 2) / C::STAGES) & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sa = base + slot * C::STAGE, sb = sa + C::OFF_B;
+                const uint32_t ta = tmem + C::SF_COL0 + (it & 1) * C::SF_COLS, tb = ta + 4 * C::CH;
+#pragma unroll
+                for (int c = 0; c < C::CH; ++c) {
+                    // w's two 128-row chunks lie side by side: 8 columns per K chunk
+                    tmem_cp_scales<true>(ta + 4 * c, smem_desc_rows16(sa + C::OFF_SFA + c * CHUNK));
+                    tmem_cp_scales<true>(tb + 8 * c, smem_desc_rows16(sa + C::OFF_SFB + c * CHUNK));
+                    tmem_cp_scales<true>(tb + 8 * c + 4, smem_desc_rows16(sa + C::OFF_SFB + C::SF_BYTES + c * CHUNK));
+                }
+                const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
+                for (int s = 0; s < steps; ++s) {
+                    const int c = FMT == MX ? s >> 1 : s;
+                    umma_fp4<FMT == MX, true>(d, smem_desc_sw128(sa + s * 32, 16, 1024),
+                                              smem_desc_sw128(sb + s * 32, 16, 1024),
+                                              idesc_fp4(256, TILE, FMT == MX, FMT == MX ? (s & 1) * 2 : 0), ta + 4 * c,
+                                              tb + 8 * c, (kt > 0 || s > 0) ? 1u : 0u);
+                }
+                umma_commit_pair(smem_u32(&empty[slot]));
+                umma_commit_pair(mapa_shared(&empty[slot], 1));
+            }
+            if (!ok) break;
+            umma_commit_pair(smem_u32(acc_full));
+            umma_commit_pair(mapa_shared(acc_full, 1));
+        }
+        if (!ok) drain_in_flight();
+    } else if (warp >= 4) {
+        const int wq = warp & 3;
+        const uint32_t stage = smem_u32(smem + C::OFF_STORE + wq * C::STORE_WARP);
+        uint32_t lt = 0;
+        bool ok = true;
+        for (int tile = first; tile < num_tiles; tile += step, ++lt) {
+            int m, n;
+            tile_at(p, tile, m, n);
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, lt & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + ((lt & 1) ? C::ACC1 : 0) + ((uint32_t)(wq * 32) << 16);
+            const int row0 = m * TILE + (int)rank * 128 + wq * 32;      // this warp's first row
+            // 32 columns from chunk `c` of the tile, held in v, to y
+            auto store = [&](int c, const uint32_t (&v)[32]) {
+                const int col = n * TILE + c * 32;
+                if (col >= p.N || row0 >= p.M) return;                  // uniform over the warp
+                const bool whole = col + 32 <= p.N;
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float b0 = 0.f, b1 = 0.f;
+                    if (p.bias) {
+                        if (whole || col + 2 * i < p.N) b0 = __bfloat162float(__ldg(p.bias + col + 2 * i));
+                        if (whole || col + 2 * i + 1 < p.N) b1 = __bfloat162float(__ldg(p.bias + col + 2 * i + 1));
+                    }
+                    w[i] = bf2u(__floats2bfloat162_rn(fmaf(__uint_as_float(v[2 * i]), p.t, b0),
+                                                      fmaf(__uint_as_float(v[2 * i + 1]), p.t, b1)));
+                }
+                // the warp's 32 x 64-byte rows through shared memory (16-byte piece q of row r
+                // at q ^ ((r >> 1) & 3): 8 lanes cover all banks either way), then whole rows out
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 +
+                                                                                  ((q ^ ((lane >> 1) & 3)) << 4)),
+                                 "r"(w[4 * q]), "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                                 : "memory");
+                __syncwarp();
+                if (p.wide && whole) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 8 * k + (lane >> 2), q = lane & 3;
+                        uint4 o;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                                     : "r"(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4))
+                                     : "memory");
+                        if (row0 + r < p.M) *reinterpret_cast<uint4 *>(p.y + (int64_t)(row0 + r) * p.ldy + col + 8 * q) = o;
+                    }
+                } else {
+                    const int rows = min(32, p.M - row0);
+                    if (col + lane < p.N) {
+                        for (int r = 0; r < rows; ++r) {
+                            uint16_t o;
+                            asm volatile("ld.shared.u16 %0, [%1];"
+                                         : "=h"(o)
+                                         : "r"(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2)
+                                         : "memory");
+                            reinterpret_cast<uint16_t *>(p.y)[(int64_t)(row0 + r) * p.ldy + col + lane] = o;
+                        }
+                    }
+                }
+                __syncwarp();
+            };
+            // the shared columns first (tensor memory 160..255: the end of accumulator 0, the
+            // start of accumulator 1), then the next tile may start
+            const int c0 = (lt & 1) ? 0 : C::ACC1 / 32;
+            uint32_t v0[32], v1[32], v2[32];
+            tmem_ld32(acc + c0 * 32, v0);
+            tmem_ld32(acc + c0 * 32 + 32, v1);
+            tmem_ld32(acc + c0 * 32 + 64, v2);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(acc_free, 0));
+            store(c0, v0);
+            store(c0 + 1, v1);
+            store(c0 + 2, v2);
+#pragma unroll 1
+            for (int c = 0; c < TILE / 32 - 3; ++c) {
+                const int cc = (lt & 1) ? c + 3 : c;
+                tmem_ld32(acc + cc * 32, v0);
+                tmem_ld_wait();
+                store(cc, v0);
+            }
+            tc_fence_before();
+        }
+        if (!ok) drain_in_flight();
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();   // neither CTA leaves while the pair's MMAs or arrivals may touch it
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+template <int FMT>
+int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    using C = Pair<FMT>;
+    auto kernel = tile_kernel<FMT>;
+    CUtensorMap tx, tw, tsx, tsw;
+    H3_CHECK(make_tmap_bytes(&tx, xc->data, xc->shape[1], xc->shape[0],
+                             xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, 128));
+    H3_CHECK(make_tmap_bytes(&tw, wc->data, wc->shape[1], wc->shape[0],
+                             wc->shape[0] > 1 ? wc->strides[0] : wc->shape[1], 128, 128));
+    H3_CHECK(make_tmap_words(&tsx, p.sx, (uint64_t)p.chunks * CHUNK, (p.M + 127) / 128, C::SF_BYTES, 1));
+    H3_CHECK(make_tmap_words(&tsw, p.sw, (uint64_t)p.chunks * CHUNK, (p.N + 127) / 128, C::SF_BYTES, 2));
+    p.num_m = (p.M + TILE - 1) / TILE;
+    p.num_n = (p.N + TILE - 1) / TILE;
+    if ((int64_t)p.num_m * p.num_n > 0x3fffffff) return H3_ERR_UNSUPPORTED;
+    p.wide = aligned16(p.y) && p.ldy % 8 == 0;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = dim3(TILE_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static std::atomic<int> pairs[64];               // resident pairs per device, once known
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
+    if (pairs[dev].load() == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+            return H3_ERR_LAUNCH;
+        cfg.gridDim = dim3(2 * (num_sms() / 2));
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return H3_ERR_LAUNCH;
+        pairs[dev].store(n);
+    }
+    const int tiles = p.num_m * p.num_n, slots = pairs[dev].load();
+    cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
+    cfg.numAttrs = p.dependent ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, tsx, tsw, p) != cudaSuccess) {
+        cudaGetLastError();
+        return H3_ERR_LAUNCH;
+    }
+    return launch_status();
+}
+
+// 0 chooses per launch, 1 forces the swap form, 2 the tile form (h3_fp4_variant)
+std::atomic<int> g_variant{0};
+
 template <int FMT>
 int multiply(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    const int v = g_variant.load();
+    if (v == 2 || (v == 0 && p.M > 128)) return launch_tiles<FMT>(xc, wc, p, stream);
     if (p.M <= 16) return launch_swap<FMT, 16>(xc, wc, p, stream);
     if (p.M <= 32) return launch_swap<FMT, 32>(xc, wc, p, stream);
     if (p.M <= 64) return launch_swap<FMT, 64>(xc, wc, p, stream);
@@ -330,6 +653,11 @@ int check_product(const h3_tensor *y, const h3_tensor *xc, const h3_tensor *xs, 
 }  // namespace h3
 
 using namespace h3;
+
+extern "C" int h3_fp4_variant(int variant) {
+    if (variant < 0 || variant > 2) return -1;
+    return fp4::g_variant.exchange(variant);
+}
 
 extern "C" int h3_linear_fp4_quantized(const h3_tensor *y, const h3_tensor *x_codes, const h3_tensor *x_scales,
                                        const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias,

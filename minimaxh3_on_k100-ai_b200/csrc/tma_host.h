@@ -57,4 +57,20 @@ inline int make_tmap_bytes(CUtensorMap *map, void *base, uint64_t width, uint64_
     return r == CUDA_SUCCESS ? H3_OK : H3_ERR_BAD_LAYOUT;
 }
 
+// Rows of `width` contiguous bytes (a multiple of 16), moved in boxes of box_bytes (at
+// most 2048) x box_rows without swizzle.  Elements are 8 bytes: a box is at most 256 wide.
+inline int make_tmap_words(CUtensorMap *map, const void *base, uint64_t width, uint64_t rows, uint32_t box_bytes,
+                           uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return H3_ERR_DRIVER;
+    const cuuint64_t dims[2] = {width / 8, rows};
+    const cuuint64_t strides[1] = {width};
+    const cuuint32_t box[2] = {box_bytes / 8, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT64, 2, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? H3_OK : H3_ERR_BAD_LAYOUT;
+}
+
 }  // namespace h3

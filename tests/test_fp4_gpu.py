@@ -149,13 +149,20 @@ def _check_product(y, xv, wv, bias=None):
     assert bool((err <= bound).all()), f"error {worst:.3g} times its bound"
 
 
+@pytest.fixture(params=[1, 2], ids=["swap", "tiles"])
+def form(h3, request):
+    old = h3.load().h3_fp4_variant(request.param)
+    yield request.param
+    h3.load().h3_fp4_variant(old)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("M,N,K", [(1, 128, 256), (1, 1, 1), (1, 5120, 5120), (2, 3, 15), (15, 127, 32), (16, 128, 33),
                                    (17, 129, 64), (31, 200, 100), (32, 512, 255), (33, 256, 256), (63, 300, 257),
                                    (64, 128, 512), (65, 640, 1795), (127, 128, 320), (128, 256, 5120), (129, 130, 96),
                                    (255, 257, 1000), (256, 256, 256), (300, 1000, 768), (513, 777, 1300),
                                    (1111, 520, 2048)])
-def test_linear(h3, fmt, M, N, K):
+def test_linear(h3, form, fmt, M, N, K):
     g = torch.Generator(device=DEV).manual_seed(M + N + K)
     x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
     bias = torch.randn(N, generator=g, device=DEV).bfloat16()
@@ -170,7 +177,7 @@ def test_linear(h3, fmt, M, N, K):
     assert h3.load().h3_device_error() == 0
 
 
-def test_linear_rows_do_not_mix(h3):
+def test_linear_rows_do_not_mix(h3, form):
     """A NaN or an infinity in one row of x, or in one weight row, reaches that row or
     column of the result and no other."""
     for fmt in FORMATS:
@@ -187,7 +194,7 @@ def test_linear_rows_do_not_mix(h3):
             assert torch.equal(y[~bad], good[~bad])
 
 
-def test_linear_layouts(h3):
+def test_linear_layouts(h3, form):
     """Batched and strided x, strided out with its surroundings untouched, odd row pitch."""
     for fmt in FORMATS:
         w = _weight(h3, 333, 640, fmt, 2)
@@ -216,6 +223,20 @@ def test_linear_tensor_scales(h3):
     assert float((h3.dequantize_fp4(xq).float() - x.float()).norm() / x.float().norm()) < 0.125
 
 
+def test_linear_many_tiles(h3, form):
+    """More tiles than the GPU holds at once: both accumulators and every ring slot are reused."""
+    for fmt in FORMATS:
+        x = torch.randn(4000, 1100, device=DEV).bfloat16()
+        w = _weight(h3, 5000, 1100, fmt, 6)
+        _check_product(h3.linear_fp4(x, w), _values(h3, h3.quantize_fp4(x, fmt)), _values(h3, w))
+    assert h3.load().h3_device_error() == 0
+
+
+def test_variant_refuses_unknown_forms(h3):
+    assert h3.load().h3_fp4_variant(3) == -1 and h3.load().h3_fp4_variant(-1) == -1
+    assert h3.load().h3_fp4_variant(0) == 0
+
+
 def test_linear_empty(h3):
     w = _weight(h3, 64, 64, "mxfp4", 4)
     assert h3.linear_fp4(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV), w).shape == (0, 64)
@@ -238,7 +259,7 @@ def test_linear_refusals(h3):
         h3.linear_fp4_(torch.empty(64, 4, 2, dtype=torch.bfloat16, device=DEV).permute(2, 1, 0), x.view(2, 4, 64), w)
 
 
-def test_graph_and_streams(h3):
+def test_graph_and_streams(h3, form):
     """Captured and replayed with new inputs, and run on two streams at once."""
     w = _weight(h3, 512, 1024, "nvfp4", 5)
     xs = [torch.randn(m, 1024, device=DEV).bfloat16() for m in (4, 200)]
