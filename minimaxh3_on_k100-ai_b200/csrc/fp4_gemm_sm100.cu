@@ -16,7 +16,7 @@
 // (one 128-byte swizzle span of codes) through a 5-slot TMA ring.  Each CTA loads its 128 x
 // rows, half the tile's w rows, and the scales of its x rows and of all the w rows; the
 // leader copies both CTAs' scales to tensor memory and issues the MMAs.  Two accumulators
-// of 256 columns and the scales do not fit the 512 columns, so the accumulators share 96:
+// of 256 columns and the scales do not fit the 512 columns, so the accumulators share 128:
 // the epilogue reads those first and then lets the next tile start, so all but that read
 // overlaps the next tile's products.
 #include <math.h>
@@ -84,6 +84,15 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
                  : "memory");
     return v;
 }
+__device__ __forceinline__ void ld_shared_words(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void st_shared_words(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ void st_shared_f32(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
@@ -125,23 +134,27 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        tma_prefetch_desc(&tx);
-        tma_prefetch_desc(&tw);
+    if (warp == 0) {
         auto load_w = [&](int i) {
             const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
             uint8_t *st = smem + slot * C::STAGE_PAD;
-            mbar_expect_tx(&full[slot], C::A_BYTES + C::B_BYTES + 2 * ch * CHUNK);
-            tma_load_2d(st, &tw, &full[slot], kt * 128, n0);
-            bulk_load(st + C::A_BYTES + C::B_BYTES, p.sw + ((int64_t)blockIdx.y * p.chunks + kt * C::CH) * CHUNK,
-                      ch * CHUNK, &full[slot]);
+            if (elect_one()) {
+                mbar_expect_tx(&full[slot], C::A_BYTES + C::B_BYTES + 2 * ch * CHUNK);
+                tma_load_2d(st, &tw, &full[slot], kt * 128, n0);
+                bulk_load(st + C::A_BYTES + C::B_BYTES, p.sw + ((int64_t)blockIdx.y * p.chunks + kt * C::CH) * CHUNK,
+                          ch * CHUNK, &full[slot]);
+            }
+            __syncwarp();
         };
         auto load_x = [&](int i) {
             const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
             uint8_t *st = smem + slot * C::STAGE_PAD;
-            tma_load_2d(st + C::A_BYTES, &tx, &full[slot], kt * 128, m0);
-            bulk_load(st + C::A_BYTES + C::B_BYTES + C::SF_BYTES,
-                      p.sx + ((int64_t)(m0 >> 7) * p.chunks + kt * C::CH) * CHUNK, ch * CHUNK, &full[slot]);
+            if (elect_one()) {
+                tma_load_2d(st + C::A_BYTES, &tx, &full[slot], kt * 128, m0);
+                bulk_load(st + C::A_BYTES + C::B_BYTES + C::SF_BYTES,
+                          p.sx + ((int64_t)(m0 >> 7) * p.chunks + kt * C::CH) * CHUNK, ch * CHUNK, &full[slot]);
+            }
+            __syncwarp();
         };
         // the weights do not wait for the quantisation of x: fill the ring with them first
         const int head = min(nk, C::STAGES);
@@ -149,11 +162,11 @@ __global__ void __launch_bounds__(SWAP_THREADS)
         if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int i = 0; i < head; ++i) load_x(i);
         for (int i = head; i < nk; ++i) {
-            if (!mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, abort_flag)) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, abort_flag))) break;
             load_w(i);
             load_x(i);
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         const uint32_t base = smem_u32(smem);
         bool ok = true;
         for (int i = 0; i < nk; ++i) {
@@ -161,30 +174,38 @@ __global__ void __launch_bounds__(SWAP_THREADS)
             ok = mbar_wait(&full[slot], (i / C::STAGES) & 1, abort_flag);
             // two scale buffers: the MMAs of tile i - 2 must have read the one about to be overwritten
             if (ok && i >= 2) ok = mbar_wait(&empty[(i - 2) % C::STAGES], ((i - 2) / C::STAGES) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             const uint32_t sa = base + slot * C::STAGE_PAD, sb = sa + C::A_BYTES;
             const uint32_t ssa = sb + C::B_BYTES, ssb = ssa + C::SF_BYTES;
             const uint32_t ta = tmem + C::SF_COL0 + (i & 1) * 2 * C::SF_COLS, tb = ta + C::SF_COLS;
             const int ch = min(C::CH, p.chunks - kt * C::CH);
-            for (int c = 0; c < ch; ++c) {
-                tmem_cp_scales<false>(ta + 4 * c, smem_desc_rows16(ssa + c * CHUNK));
-                tmem_cp_scales<false>(tb + 4 * c, smem_desc_rows16(ssb + c * CHUNK));
-            }
             const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
             const uint32_t tb0 = tb + ((m0 & 127) >> 5);     // this tile's rows within the 128-row chunk
-            for (int s = 0; s < steps; ++s) {
-                const int c = FMT == MX ? s >> 1 : s;
-                const uint32_t id = FMT == MX ? (s & 1) * 2 : 0;
-                umma_fp4<FMT == MX, false>(tmem, smem_desc_sw128(sa + s * 32, 16, 1024),
-                                           smem_desc_sw128(sb + s * 32, 16, 1024),
-                                           idesc_fp4(128, BN, FMT == MX, id), ta + 4 * c, tb0 + 4 * c,
-                                           (i > 0 || s > 0) ? 1u : 0u);
+            if (elect_one()) {
+#pragma unroll
+                for (int c = 0; c < C::CH; ++c) {
+                    if (c < ch) {
+                        tmem_cp_scales<false>(ta + 4 * c, smem_desc_rows16(ssa + c * CHUNK));
+                        tmem_cp_scales<false>(tb + 4 * c, smem_desc_rows16(ssb + c * CHUNK));
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < BK / KSTEP; ++s) {
+                    const int c = FMT == MX ? s >> 1 : s;
+                    if (s < steps)
+                        umma_fp4<FMT == MX, false>(tmem, smem_desc_sw128(sa + s * 32, 16, 1024),
+                                                   smem_desc_sw128(sb + s * 32, 16, 1024),
+                                                   idesc_fp4(128, BN, FMT == MX, FMT == MX ? (s & 1) * 2 : 0),
+                                                   ta + 4 * c, tb0 + 4 * c, (i > 0 || s > 0) ? 1u : 0u);
+                }
+                umma_commit(&empty[slot]);
+                if (i == nk - 1) umma_commit(done);
             }
-            umma_commit(&empty[slot]);
+            __syncwarp();
         }
-        if (ok) umma_commit(done);
-        else drain_in_flight();
+        if (!ok) drain_in_flight();
     }
     __syncwarp();
     const bool ok = nk == 0 || __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag));
@@ -319,15 +340,16 @@ struct Pair {
     static constexpr int OFF_SFB = OFF_SFA + SF_BYTES;        // all 256 w rows: each CTA multiplies with every one
     static constexpr int STAGE = OFF_SFB + 2 * SF_BYTES;      // a multiple of 1024
     static constexpr int STAGES = 5;
-    static constexpr int STORE_WARP = 32 * 64;                // an epilogue warp's 32 rows x 32 columns
+    static constexpr int STORE = 32 * 128;                    // 32 rows x 64 columns of y, two per epilogue warp
     static constexpr int OFF_STORE = STAGES * STAGE;
-    static constexpr int OFF_BAR = OFF_STORE + 4 * STORE_WARP;
+    static constexpr int OFF_BIAS = OFF_STORE + 8 * STORE;    // the tile's bias, a copy per epilogue warp
+    static constexpr int OFF_BAR = OFF_BIAS + 4 * 512;
     static constexpr int SMEM = OFF_BAR + (2 * STAGES + 2) * 8 + 16 + 1024;
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
-    // Tensor memory: two 256-column accumulators sharing 96 columns, and two buffers of
+    // Tensor memory: two 256-column accumulators sharing 128 columns, and two buffers of
     // scales (4 columns per 128 rows and chunk: 4 CH of x, 8 CH of w)
-    static constexpr int ACC1 = 160;
-    static constexpr int SF_COL0 = 416;
+    static constexpr int ACC1 = 128;
+    static constexpr int SF_COL0 = 384;
     static constexpr int SF_COLS = 12 * CH;
     static_assert(SF_COL0 + 2 * SF_COLS <= 512 && ACC1 + TILE <= SF_COL0, "tensor memory");
 };
@@ -343,7 +365,8 @@ __device__ __forceinline__ void tile_at(const Params &p, int tile, int &m, int &
 template <int FMT>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw,
-                const __grid_constant__ CUtensorMap tsx, const __grid_constant__ CUtensorMap tsw, Params p) {
+                const __grid_constant__ CUtensorMap tsx, const __grid_constant__ CUtensorMap tsw,
+                const __grid_constant__ CUtensorMap ty, Params p) {
     using C = Pair<FMT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -378,11 +401,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0 && lane == 0) {
-        tma_prefetch_desc(&tx);
-        tma_prefetch_desc(&tw);
-        tma_prefetch_desc(&tsx);
-        tma_prefetch_desc(&tsw);
+    if (warp == 0) {
+        if (elect_one()) {
+            tma_prefetch_desc(&tx);
+            tma_prefetch_desc(&tw);
+            tma_prefetch_desc(&tsx);
+            tma_prefetch_desc(&tsw);
+        }
         if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
         uint32_t it = 0;
         bool ok = true;
@@ -391,16 +416,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             tile_at(p, tile, m, n);
             for (int kt = 0; kt < p.ktiles; ++kt, ++it) {
                 const uint32_t slot = it % C::STAGES;
-                ok = mbar_wait(&empty[slot], ((it / C::STAGES) & 1) ^ 1, abort_flag);
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((it / C::STAGES) & 1) ^ 1, abort_flag));
                 if (!ok) break;
-                // both CTAs' bytes are counted on the leader's barrier
-                const uint32_t bar = mapa_shared(&full[slot], 0);
-                if (rank == 0) mbar_expect_tx(&full[slot], 2 * C::STAGE);
-                uint8_t *st = smem + slot * C::STAGE;
-                tma_load_2d_pair(st, &tx, bar, kt * 128, m * TILE + (int)rank * 128);
-                tma_load_2d_pair(st + C::OFF_B, &tw, bar, kt * 128, n * TILE + (int)rank * 128);
-                tma_load_2d_pair(st + C::OFF_SFA, &tsx, bar, kt * (C::SF_BYTES / 8), 2 * m + (int)rank);
-                tma_load_2d_pair(st + C::OFF_SFB, &tsw, bar, kt * (C::SF_BYTES / 8), 2 * n);
+                if (elect_one()) {
+                    // both CTAs' bytes are counted on the leader's barrier
+                    const uint32_t bar = mapa_shared(&full[slot], 0);
+                    if (rank == 0) mbar_expect_tx(&full[slot], 2 * C::STAGE);
+                    uint8_t *st = smem + slot * C::STAGE;
+                    tma_load_2d_pair(st, &tx, bar, kt * 128, m * TILE + (int)rank * 128);
+                    tma_load_2d_pair(st + C::OFF_B, &tw, bar, kt * 128, n * TILE + (int)rank * 128);
+                    tma_load_2d_pair(st + C::OFF_SFA, &tsx, bar, kt * (C::SF_BYTES / 8), 2 * m + (int)rank);
+                    tma_load_2d_pair(st + C::OFF_SFB, &tsw, bar, kt * (C::SF_BYTES / 8), 2 * n);
+                }
+                __syncwarp();
             }
         }
         // the leader's last commits arrive here: none may land after this CTA has gone
@@ -409,13 +437,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             const uint32_t u = it - 1 - i;
             ok = mbar_wait(&empty[u % C::STAGES], (u / C::STAGES) & 1, abort_flag);
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+        // the whole warp runs this; one lane issues
         const uint32_t base = smem_u32(smem);
         uint32_t it = 0, lt = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles && ok; tile += step, ++lt) {
             // the accumulator two tiles back has been read wholly before the last one's shared columns
-            if (lt > 0) ok = mbar_wait_cluster(acc_free, (lt - 1) & 1, abort_flag);
+            if (lt > 0) ok = __all_sync(0xffffffffu, mbar_wait_cluster(acc_free, (lt - 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + ((lt & 1) ? C::ACC1 : 0);
@@ -425,120 +454,133 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 // two scale buffers: the MMAs two K tiles back must have read this one
                 if (ok && it >= 2)
                     ok = mbar_wait(&empty[(it - 2) % C::STAGES], ((it - 2) / C::STAGES) & 1, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t sa = base + slot * C::STAGE, sb = sa + C::OFF_B;
                 const uint32_t ta = tmem + C::SF_COL0 + (it & 1) * C::SF_COLS, tb = ta + 4 * C::CH;
-#pragma unroll
-                for (int c = 0; c < C::CH; ++c) {
-                    // w's two 128-row chunks lie side by side: 8 columns per K chunk
-                    tmem_cp_scales<true>(ta + 4 * c, smem_desc_rows16(sa + C::OFF_SFA + c * CHUNK));
-                    tmem_cp_scales<true>(tb + 8 * c, smem_desc_rows16(sa + C::OFF_SFB + c * CHUNK));
-                    tmem_cp_scales<true>(tb + 8 * c + 4, smem_desc_rows16(sa + C::OFF_SFB + C::SF_BYTES + c * CHUNK));
-                }
                 const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
-                for (int s = 0; s < steps; ++s) {
-                    const int c = FMT == MX ? s >> 1 : s;
-                    umma_fp4<FMT == MX, true>(d, smem_desc_sw128(sa + s * 32, 16, 1024),
-                                              smem_desc_sw128(sb + s * 32, 16, 1024),
-                                              idesc_fp4(256, TILE, FMT == MX, FMT == MX ? (s & 1) * 2 : 0), ta + 4 * c,
-                                              tb + 8 * c, (kt > 0 || s > 0) ? 1u : 0u);
+                if (elect_one()) {
+#pragma unroll
+                    for (int c = 0; c < C::CH; ++c) {
+                        // w's two 128-row chunks lie side by side: 8 columns per K chunk
+                        tmem_cp_scales<true>(ta + 4 * c, smem_desc_rows16(sa + C::OFF_SFA + c * CHUNK));
+                        tmem_cp_scales<true>(tb + 8 * c, smem_desc_rows16(sa + C::OFF_SFB + c * CHUNK));
+                        tmem_cp_scales<true>(tb + 8 * c + 4,
+                                             smem_desc_rows16(sa + C::OFF_SFB + C::SF_BYTES + c * CHUNK));
+                    }
+#pragma unroll
+                    for (int s = 0; s < BK / KSTEP; ++s) {
+                        const int c = FMT == MX ? s >> 1 : s;
+                        if (s < steps)
+                            umma_fp4<FMT == MX, true>(d, smem_desc_sw128(sa + s * 32, 16, 1024),
+                                                      smem_desc_sw128(sb + s * 32, 16, 1024),
+                                                      idesc_fp4(256, TILE, FMT == MX, FMT == MX ? (s & 1) * 2 : 0),
+                                                      ta + 4 * c, tb + 8 * c, (kt > 0 || s > 0) ? 1u : 0u);
+                    }
+                    umma_commit_pair(smem_u32(&empty[slot]));
+                    umma_commit_pair(mapa_shared(&empty[slot], 1));
                 }
-                umma_commit_pair(smem_u32(&empty[slot]));
-                umma_commit_pair(mapa_shared(&empty[slot], 1));
+                __syncwarp();
             }
             if (!ok) break;
-            umma_commit_pair(smem_u32(acc_full));
-            umma_commit_pair(mapa_shared(acc_full, 1));
+            if (elect_one()) {
+                umma_commit_pair(smem_u32(acc_full));
+                umma_commit_pair(mapa_shared(acc_full, 1));
+            }
+            __syncwarp();
         }
         if (!ok) drain_in_flight();
     } else if (warp >= 4) {
         const int wq = warp & 3;
-        const uint32_t stage = smem_u32(smem + C::OFF_STORE + wq * C::STORE_WARP);
+        uint8_t *buf0 = smem + C::OFF_STORE + wq * 2 * C::STORE;
+        const uint32_t bias = smem_u32(smem + C::OFF_BIAS + wq * 512);
         uint32_t lt = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles; tile += step, ++lt) {
             int m, n;
             tile_at(p, tile, m, n);
+            const int row0 = m * TILE + (int)rank * 128 + wq * 32;      // this warp's first row
+            if (p.bias) {
+                uint16_t b[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int col = n * TILE + lane * 8 + i;
+                    b[i] = col < p.N ? __ldg(reinterpret_cast<const uint16_t *>(p.bias) + col) : (uint16_t)0;
+                }
+                st_shared_words(bias + lane * 16, b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16,
+                                b[4] | (uint32_t)b[5] << 16, b[6] | (uint32_t)b[7] << 16);
+                __syncwarp();
+            }
             ok = __all_sync(0xffffffffu, mbar_wait(acc_full, lt & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((lt & 1) ? C::ACC1 : 0) + ((uint32_t)(wq * 32) << 16);
-            const int row0 = m * TILE + (int)rank * 128 + wq * 32;      // this warp's first row
-            // 32 columns from chunk `c` of the tile, held in v, to y
-            auto store = [&](int c, const uint32_t (&v)[32]) {
-                const int col = n * TILE + c * 32;
-                if (col >= p.N || row0 >= p.M) return;                  // uniform over the warp
-                const bool whole = col + 32 <= p.N;
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float b0 = 0.f, b1 = 0.f;
-                    if (p.bias) {
-                        if (whole || col + 2 * i < p.N) b0 = __bfloat162float(__ldg(p.bias + col + 2 * i));
-                        if (whole || col + 2 * i + 1 < p.N) b1 = __bfloat162float(__ldg(p.bias + col + 2 * i + 1));
-                    }
-                    w[i] = bf2u(__floats2bfloat162_rn(fmaf(__uint_as_float(v[2 * i]), p.t, b0),
-                                                      fmaf(__uint_as_float(v[2 * i + 1]), p.t, b1)));
+            // 64 columns at a time, the shared ones first (the end of accumulator 0, the start
+            // of accumulator 1); once they are in registers the next tile may start
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const int c0 = ((lt & 1) ? i : i ^ 2) * 64, col = n * TILE + c0;
+                uint32_t v[2][32];
+                tmem_ld32(acc + c0, v[0]);
+                tmem_ld32(acc + c0 + 32, v[1]);
+                tmem_ld_wait();
+                if (i == 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(mapa_shared(acc_free, 0));
                 }
-                // the warp's 32 x 64-byte rows through shared memory (16-byte piece q of row r
-                // at q ^ ((r >> 1) & 3): 8 lanes cover all banks either way), then whole rows out
+                if (col >= p.N || row0 >= p.M) continue;                // uniform over the warp
+                uint32_t w[32];
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 +
-                                                                                  ((q ^ ((lane >> 1) & 3)) << 4)),
-                                 "r"(w[4 * q]), "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
-                                 : "memory");
-                __syncwarp();
-                if (p.wide && whole) {
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = 8 * k + (lane >> 2), q = lane & 3;
-                        uint4 o;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
-                                     : "r"(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4))
-                                     : "memory");
-                        if (row0 + r < p.M) *reinterpret_cast<uint4 *>(p.y + (int64_t)(row0 + r) * p.ldy + col + 8 * q) = o;
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t b[4] = {0, 0, 0, 0};
+                        if (p.bias) ld_shared_words(bias + (c0 + 32 * h + 8 * q) * 2, b);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[16 * h + 4 * q + e] = bf2u(
+                                __floats2bfloat162_rn(fmaf(__uint_as_float(v[h][8 * q + 2 * e]), p.t, blo(b[e])),
+                                                      fmaf(__uint_as_float(v[h][8 * q + 2 * e + 1]), p.t, bhi(b[e]))));
+                    }
+                uint8_t *buf = buf0 + (i & 1) * C::STORE;
+                if (p.wide) {
+                    if (lane == 0) tma_store_wait_read_1();              // the store two blocks back has read it
+                    __syncwarp();
+                }
+                // 16-byte piece q of row r at q ^ (r & 7): the layout the TMA store reads
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    st_shared_words(smem_u32(buf) + lane * 128 + ((q ^ (lane & 7)) << 4), w[4 * q], w[4 * q + 1],
+                                    w[4 * q + 2], w[4 * q + 3]);
+                if (p.wide) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&ty, buf, col, row0);               // clipped at y's edges
+                        tma_store_commit();
                     }
                 } else {
+                    // rows too odd for TMA: two columns per lane, a row at a time
+                    __syncwarp();
                     const int rows = min(32, p.M - row0);
-                    if (col + lane < p.N) {
-                        for (int r = 0; r < rows; ++r) {
-                            uint16_t o;
-                            asm volatile("ld.shared.u16 %0, [%1];"
-                                         : "=h"(o)
-                                         : "r"(stage + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2)
-                                         : "memory");
-                            reinterpret_cast<uint16_t *>(p.y)[(int64_t)(row0 + r) * p.ldy + col + lane] = o;
-                        }
+                    for (int r = 0; r < rows; ++r) {
+                        uint32_t o;
+                        asm volatile("ld.shared.b32 %0, [%1];"
+                                     : "=r"(o)
+                                     : "r"(smem_u32(buf) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)
+                                     : "memory");
+                        uint16_t *dst = reinterpret_cast<uint16_t *>(p.y) + (int64_t)(row0 + r) * p.ldy + col + 2 * lane;
+                        if (col + 2 * lane < p.N) dst[0] = (uint16_t)o;
+                        if (col + 2 * lane + 1 < p.N) dst[1] = (uint16_t)(o >> 16);
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
-            };
-            // the shared columns first (tensor memory 160..255: the end of accumulator 0, the
-            // start of accumulator 1), then the next tile may start
-            const int c0 = (lt & 1) ? 0 : C::ACC1 / 32;
-            uint32_t v0[32], v1[32], v2[32];
-            tmem_ld32(acc + c0 * 32, v0);
-            tmem_ld32(acc + c0 * 32 + 32, v1);
-            tmem_ld32(acc + c0 * 32 + 64, v2);
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(acc_free, 0));
-            store(c0, v0);
-            store(c0 + 1, v1);
-            store(c0 + 2, v2);
-#pragma unroll 1
-            for (int c = 0; c < TILE / 32 - 3; ++c) {
-                const int cc = (lt & 1) ? c + 3 : c;
-                tmem_ld32(acc + cc * 32, v0);
-                tmem_ld_wait();
-                store(cc, v0);
             }
             tc_fence_before();
         }
+        if (p.wide && lane == 0) tma_store_wait_all();
         if (!ok) drain_in_flight();
     }
     __syncwarp();
@@ -566,6 +608,13 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
     p.num_n = (p.N + TILE - 1) / TILE;
     if ((int64_t)p.num_m * p.num_n > 0x3fffffff) return H3_ERR_UNSUPPORTED;
     p.wide = aligned16(p.y) && p.ldy % 8 == 0;
+    CUtensorMap ty = tx;                             // not used where rows are too odd for it
+    if (p.wide) {
+        const cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M};
+        const cuuint64_t strides[1] = {(cuuint64_t)(p.M > 1 ? p.ldy : (p.N + 7) / 8 * 8) * 2};
+        const cuuint32_t box[2] = {64, 32};
+        H3_CHECK(make_tmap_bf16(&ty, p.y, 2, dims, strides, box));
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -594,7 +643,7 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
     const int tiles = p.num_m * p.num_n, slots = pairs[dev].load();
     cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
     cfg.numAttrs = p.dependent ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, tsx, tsw, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, tsx, tsw, ty, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;
     }

@@ -139,6 +139,19 @@ __device__ __forceinline__ void drain_in_flight() {
     }
 }
 
+// One lane of a converged warp.  Code around it stays warp-uniform, so that descriptors
+// and addresses are kept in uniform registers, where tcgen05 and TMA instructions take
+// them from; inside a `lane == 0` branch each operand is moved there one by one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 // ----------------------------------------------------------------------------
 // fences and named barriers
 // ----------------------------------------------------------------------------
@@ -208,6 +221,10 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, const void 
 }
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// all but the latest store have read their shared memory
+__device__ __forceinline__ void tma_store_wait_read_1() {
+    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+}
 __device__ __forceinline__ void tma_store_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
