@@ -186,6 +186,22 @@ int h3_mha(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, const h
 int h3_mha_scatter(const h3_tensor *dsts, int32_t ndst, const h3_tensor *q, const h3_tensor *k,
                    const h3_tensor *v, float scale, void *stream);
 
+/* Cross attention to an encoder's states: q, out [B,Sq,H,128]; k, v [B or 1,Sk,Hkv,128]
+ * (batch 1 or batch stride 0: the same states for every sample), H a multiple of Hkv
+ * (query head h reads key/value head h / (H / Hkv)); lengths [B] I64 on the device, the
+ * number of states of each sample (clamped to [0, Sk]), or NULL for Sk.  Non-causal,
+ * fp32 softmax and accumulation, P rounded to BF16.  States behind a sample's length are
+ * not read into a result whatever they hold; a sample without states, and a row whose
+ * scores are all -inf, gets zeros.  scale positive and finite.  Layout rules of h3_mha.
+ * No reference counterpart (its attention, h3_mha, has one key length and equal heads). */
+int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, const h3_tensor *v,
+                       const h3_tensor *lengths, float scale, void *stream);
+
+/* Form of h3_cross_attention: 0 = chosen per launch, 1 = rows form (few rows per key/value
+ * head, keys split over a cluster), 2 = 128-row tiles.  Returns the previous setting, or -1
+ * for a value outside 0..2 (setting unchanged).  A tuning and test hook. */
+int h3_cross_attention_variant(int variant);
+
 /* ---------------- projections (BF16 in/out, fp32 accumulate) ---------------- */
 
 /* y [M,N] = x [M,K] * w[N,K]^T.  Rows of x, w, y contiguous (inner stride 1),

@@ -66,6 +66,8 @@ SIGNATURES = {
     "h3_timestep_embedding": [P, P, _F, _V],
     "h3_mha": [P, P, P, P, _F, _V],
     "h3_mha_scatter": [P, _I, P, P, P, _F, _V],
+    "h3_cross_attention": [P, P, P, P, P, _F, _V],
+    "h3_cross_attention_variant": [ctypes.c_int],
     "h3_linear": [P, P, P, _V],
     "h3_linear_swiglu": [P, P, P, _V],
     "h3_linear_gated_residual": [P, P, P, P, P, _V],

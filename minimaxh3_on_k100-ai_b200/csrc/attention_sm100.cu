@@ -64,6 +64,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "attn_math.cuh"
 #include "h3_abi_util.h"
 #include "h3_common.cuh"
 #include "sm100_ptx.cuh"
@@ -166,49 +167,6 @@ struct Params {
     __nv_bfloat16 *dst[H3_EXCHANGE_MAX_RANKS];
 };
 
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ void st_global_v4(void *ptr, const uint4 &v) {
-    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(ptr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-}
-
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Blackwell packed fp32 pairs (fma.rn.f32x2 / add.rn.f32x2) and the 3-input
-// max halve the issue slots of the softmax's per-element fp32 work.
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t pk2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void up2(uint64_t v, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // 2^x for a pair of values on the FMA pipe (packed fp32x2): x = n + f with
 // n = round(x) (the 1.5*2^23 addition leaves n in the low mantissa bits), 2^f by
 // a degree-3 polynomial on [-1/2, 1/2] (Lawson minimax fit, max relative error
@@ -235,20 +193,6 @@ __device__ __forceinline__ float bf16_round_up(float x) {
     uint32_t u = __float_as_uint(x);
     if ((u & 0xFFFFu) != 0u && !(u >> 31)) u += 0x10000u;   // positive with dropped bits: up
     return __uint_as_float(u & 0xFFFF0000u);                 // negative: truncation rounds up
-}
-
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t *>(&v);
-}
-
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-
-// byte offset of 16-byte chunk `chunk` (0..7) of row `row` inside a 128B-swizzled 64-column half
-__device__ __forceinline__ uint32_t swz(int row, int chunk) {
-    return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
 // The work of one CTA on NQT (1 or 2) Q tiles starting at row q0 of (batch b, head h).

@@ -27,6 +27,7 @@ __all__ = [
     "h3_ln_modulate", "h3_ln_modulate_", "h3_rope", "h3_rope_", "h3_gated_residual", "h3_gated_residual_",
     "h3_gated_residual_rms_modulate", "h3_gated_residual_rms_modulate_", "h3_qk_norm_rope_",
     "h3_rope_cache", "h3_rope_cache_sectioned", "rope_powers", "timestep_embedding", "mha", "mha_",
+    "cross_attention", "cross_attention_",
     "linear", "linear_", "linear_swiglu", "linear_gated_residual", "pack_gate_up",
     "linear_f32", "linear_f32_", "gather_rows", "gather_rows_", "index_copy_rows_", "silu", "silu_",
     "linear_qkv_norm_rope_", "linear_gated_residual_sq", "h3_rms_modulate_sq_",
@@ -185,6 +186,25 @@ def mha_(out, q, k, v, scale=None):
 
 def mha(q, k, v, scale=None):
     return mha_(torch.empty(q.shape, dtype=q.dtype, device=q.device), q, k, v, scale)
+
+
+def cross_attention_(out, q, k, v, lengths=None, scale=None):
+    """Attention of q [B,Sq,H,D] to an encoder's states k, v [B or 1,Sk,Hkv,D] of another
+    length, into out [B,Sq,H,D] (D = 128, H a multiple of Hkv).  ``lengths`` [B] int64 on
+    the device: the number of states of each sample; what lies behind is ignored whatever
+    it holds, and a sample with none gets zeros.  A batch of 1 (or an expanded one) is
+    shared by all samples.  No reference counterpart."""
+    require_cuda(out, q, k, v, lengths)
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if not 0.0 < scale <= 3e38:
+        raise ValueError(f"the scale must be positive and finite, got {scale}")
+    call("h3_cross_attention", desc(out), desc(q), desc(k), desc(v), desc(lengths), scale, stream_of(q))
+    return out
+
+
+def cross_attention(q, k, v, lengths=None, scale=None):
+    return cross_attention_(torch.empty(q.shape, dtype=q.dtype, device=q.device), q, k, v, lengths, scale)
 
 
 # ---------------------------------------------------------------------------
