@@ -334,13 +334,13 @@ int h3_quantize_fp4(const h3_tensor *codes, const h3_tensor *scales, const h3_te
 int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tensor *scales, int32_t format,
                       float tensor_scale, void *stream);
 
-/* y [M,N] = bf16(xq wq^T + bias): x [M,K] BF16 is quantised into x_codes / x_scales
- * (caller-owned workspace of x's 4-bit shapes, any contents) and multiplied with the
- * 4-bit weight [N,K] of the same format; fp32 accumulation, one rounding.  bias [N] BF16
- * or NULL.  Any M, N, K >= 1 (K at most 2^24); rows of y and x contiguous. */
-int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *x_codes, const h3_tensor *x_scales,
-                  const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int32_t format,
-                  float x_tensor_scale, float w_tensor_scale, void *stream);
+/* y [M,N] = bf16(xq wq^T + bias): x [M,K] BF16 is quantised into the workspace (U8, 1-D,
+ * 16-byte aligned, any contents, at least as many bytes as x's codes and scales together)
+ * and multiplied with the 4-bit weight [N,K] of the same format; fp32 accumulation, one
+ * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1. */
+int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace, const h3_tensor *w_codes,
+                  const h3_tensor *w_scales, const h3_tensor *bias, int32_t format, float x_tensor_scale,
+                  float w_tensor_scale, void *stream);
 
 /* Form of the 4-bit projections: 0 = chosen per launch, 1 = weight rows as the M side and
  * K split over a cluster (few rows of x), 2 = CTA-pair 256 x 256 tiles.  The forms add in

@@ -41,6 +41,7 @@ class H3Tensor(ctypes.Structure):
 
 
 P = ctypes.POINTER(H3Tensor)
+D = ctypes.c_void_p      # a descriptor by reference, or its bytes (``packed``)
 _F = ctypes.c_float
 _V = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -66,7 +67,7 @@ SIGNATURES = {
     "h3_timestep_embedding": [P, P, _F, _V],
     "h3_mha": [P, P, P, P, _F, _V],
     "h3_mha_scatter": [P, _I, P, P, P, _F, _V],
-    "h3_cross_attention": [P, P, P, P, P, _F, _V],
+    "h3_cross_attention": [D, D, D, D, D, _F, _V],
     "h3_cross_attention_variant": [ctypes.c_int],
     "h3_linear": [P, P, P, _V],
     "h3_linear_swiglu": [P, P, P, _V],
@@ -79,11 +80,11 @@ SIGNATURES = {
     "h3_linear_gated_residual_rms_modulate_noalloc": [P, P, P, P, P, P, P, P, P, _F, _V],
     "h3_pack_gate_up": [P, P, _V],
     "h3_linear_qkv_norm_rope": [P, P, P, P, P, _I, P, P, P, P, _F, _V],
-    "h3_quantize_fp4": [P, P, P, _I, _F, _V],
-    "h3_dequantize_fp4": [P, P, P, _I, _F, _V],
+    "h3_quantize_fp4": [D, D, D, _I, _F, _V],
+    "h3_dequantize_fp4": [D, D, D, _I, _F, _V],
     "h3_fp4_variant": [ctypes.c_int],
-    "h3_linear_fp4": [P, P, P, P, P, P, P, _I, _F, _F, _V],
-    "h3_linear_fp4_quantized": [P, P, P, P, P, P, ctypes.c_int64, _I, _F, _F, _V],
+    "h3_linear_fp4": [D, D, D, D, D, D, _I, _F, _F, _V],
+    "h3_linear_fp4_quantized": [D, D, D, D, D, D, ctypes.c_int64, _I, _F, _F, _V],
     "h3_linear_f32": [P, P, P, P, _V],
     "h3_gather_rows": [P, P, P, _V],
     "h3_index_copy_rows": [P, P, P, _V],
@@ -134,12 +135,21 @@ def desc(t: torch.Tensor | None) -> H3Tensor | None:
     return H3Tensor.from_buffer_copy(_PACK[n](t.data_ptr(), *t.shape, *t.stride(), n, code))
 
 
-def desc_rows(ptr: int, dtype: torch.dtype, *shape: int) -> H3Tensor:
-    """The descriptor of a contiguous tensor at ``ptr`` (a piece of a workspace)."""
-    strides = [1] * len(shape)
-    for i in range(len(shape) - 1, 0, -1):
-        strides[i - 1] = strides[i] * shape[i]
-    return H3Tensor.from_buffer_copy(_PACK[len(shape)](ptr, *shape, *strides, len(shape), _DTYPES[dtype]))
+def packed(t: torch.Tensor | None) -> bytes | None:
+    """``desc`` as bytes, for the entry points that take ``D`` arguments (0.3 us less each)."""
+    if t is None:
+        return None
+    n = t.dim()
+    code = _DTYPES.get(t.dtype)
+    if n > 4 or code is None:
+        desc(t)   # raises
+    return _PACK[n](t.data_ptr(), *t.shape, *t.stride(), n, code)
+
+
+def packed_bytes(ptr: int, shape: tuple, strides: tuple) -> bytes:
+    """The descriptor of a byte tensor given by its parts (a piece of a buffer)."""
+    n = len(shape)
+    return _PACK[n](ptr, *shape, *strides, n, 4)
 
 
 def ref(d: H3Tensor | None):

@@ -721,20 +721,31 @@ extern "C" int h3_linear_fp4_quantized(const h3_tensor *y, const h3_tensor *x_co
                              : fp4::multiply<fp4::NV>(x_codes, w_codes, p, (cudaStream_t)stream);
 }
 
-extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *x_codes,
-                             const h3_tensor *x_scales, const h3_tensor *w_codes, const h3_tensor *w_scales,
-                             const h3_tensor *bias, int32_t format, float x_tensor_scale, float w_tensor_scale,
-                             void *stream) {
+extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace,
+                             const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int32_t format,
+                             float x_tensor_scale, float w_tensor_scale, void *stream) {
     H3_CHECK(check_bf16(x));
-    if (x->ndim != 2) return H3_ERR_BAD_SHAPE;
+    H3_CHECK(check_desc(workspace, H3_U8));
+    if (x->ndim != 2 || x->shape[1] < 1) return H3_ERR_BAD_SHAPE;
+    if (format != fp4::MX && format != fp4::NV) return H3_ERR_UNSUPPORTED;
+    const int64_t rows = x->shape[0], cols = x->shape[1];
+    if (rows > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
+    // x in 4 bits: its codes, then its scales
+    const int64_t pitch = fp4::code_pitch(cols), groups = (rows + 127) / 128, chunks = fp4::scale_chunks(format, cols);
+    if (workspace->ndim != 1 || workspace->shape[0] < rows * pitch + groups * chunks * fp4::CHUNK)
+        return H3_ERR_BAD_SHAPE;
+    if (rows > 0 && (workspace->strides[0] != 1 || !aligned16(workspace->data))) return H3_ERR_BAD_LAYOUT;
+    uint8_t *at = static_cast<uint8_t *>(workspace->data);
+    const h3_tensor xc = {at, {rows, pitch}, {pitch, 1}, 2, H3_U8};
+    const h3_tensor xs = {at + rows * pitch, {groups, chunks, fp4::CHUNK}, {chunks * fp4::CHUNK, fp4::CHUNK, 1}, 3, H3_U8};
     fp4::Params p{};
-    H3_CHECK(fp4::check_product(y, x_codes, x_scales, w_codes, w_scales, bias, x->shape[0], x->shape[1], format,
-                                x_tensor_scale, w_tensor_scale, &p));
+    H3_CHECK(fp4::check_product(y, &xc, &xs, w_codes, w_scales, bias, rows, cols, format, x_tensor_scale,
+                                w_tensor_scale, &p));
     if (p.M == 0 || p.N == 0) return H3_OK;
-    H3_CHECK(fp4::quantize(x_codes, x_scales, x, format, x_tensor_scale, (cudaStream_t)stream));
+    H3_CHECK(fp4::quantize(&xc, &xs, x, format, x_tensor_scale, (cudaStream_t)stream));
     p.dependent = 1;
-    return format == fp4::MX ? fp4::multiply<fp4::MX>(x_codes, w_codes, p, (cudaStream_t)stream)
-                             : fp4::multiply<fp4::NV>(x_codes, w_codes, p, (cudaStream_t)stream);
+    return format == fp4::MX ? fp4::multiply<fp4::MX>(&xc, w_codes, p, (cudaStream_t)stream)
+                             : fp4::multiply<fp4::NV>(&xc, w_codes, p, (cudaStream_t)stream);
 }
 
 // device error word of this translation unit (bounded waits of the products)

@@ -15,11 +15,10 @@ No counterpart in the reference.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
 
 import torch
 
-from ._lib import call, desc, desc_rows, require_cuda, stream_of
+from ._lib import call, packed, packed_bytes, require_cuda, stream_of
 
 __all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_fp4", "quantize_fp4_", "dequantize_fp4",
            "dequantize_fp4_", "pack_fp4", "unpack_fp4", "linear_fp4", "linear_fp4_"]
@@ -46,17 +45,50 @@ def _check_tensor_scale(fmt: str, scale: float) -> float:
     return scale
 
 
-@dataclass
 class Fp4Tensor:
     """A matrix of ``rows`` x ``cols`` 4-bit values: ``codes`` uint8
     [rows, ceil(cols/32)*16] (two codes a byte) and ``scales`` uint8
-    [ceil(rows/128), ceil(blocks/4), 512], as the products read them."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    cols: int
-    format: str
-    tensor_scale: float = 1.0
+    [ceil(rows/128), ceil(blocks/4), 512], as the products read them.  Immutable but for
+    its contents: the descriptors the entry points take are made once."""
+
+    __slots__ = ("rows", "cols", "format", "tensor_scale", "d_codes", "d_scales", "_buffer", "_codes", "_scales")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, format: str,
+                 tensor_scale: float = 1.0):
+        _check_format(format)
+        self.rows, self.cols, self.format = rows, cols, format
+        self.tensor_scale = _check_tensor_scale(format, tensor_scale)
+        if codes.device != scales.device:
+            raise ValueError("codes and scales must be on the same device")
+        self._codes, self._scales, self._buffer = codes, scales, codes
+        self.d_codes, self.d_scales = packed(codes), packed(scales)
+
+    @classmethod
+    def _uninitialised(cls, like: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
+        """On ``like``'s device, codes and scales in one allocation."""
+        self = cls.__new__(cls)
+        self.rows, self.cols, self.format, self.tensor_scale = rows, cols, format, tensor_scale
+        pitch, groups, chunks = _layout(rows, cols, format)
+        self._buffer = buf = like.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)
+        at = buf.data_ptr()
+        self.d_codes = packed_bytes(at, (rows, pitch), (pitch, 1))
+        self.d_scales = packed_bytes(at + rows * pitch, (groups, chunks, 512), (chunks * 512, 512, 1))
+        self._codes = self._scales = None
+        return self
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            pitch, _, _ = _layout(self.rows, self.cols, self.format)
+            self._codes = self._buffer[: self.rows * pitch].view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            pitch, groups, chunks = _layout(self.rows, self.cols, self.format)
+            self._scales = self._buffer[self.rows * pitch:].view(groups, chunks, 512)
+        return self._scales
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -64,19 +96,25 @@ class Fp4Tensor:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._buffer.device
+
+    def __repr__(self) -> str:
+        return f"Fp4Tensor({self.rows} x {self.cols}, {self.format}, tensor_scale={self.tensor_scale}, {self.device})"
+
+
+def _layout(rows: int, cols: int, fmt: str) -> tuple[int, int, int]:
+    """Bytes of a row of codes, 128-row groups and chunks per group of the scales."""
+    per_chunk = 128 if fmt == "mxfp4" else 64
+    return (cols + 31) // 32 * 16, (rows + 127) // 128, (cols + per_chunk - 1) // per_chunk
 
 
 def fp4_empty(rows: int, cols: int, format: str = "nvfp4", tensor_scale: float = 1.0, device="cuda") -> Fp4Tensor:
-    """An uninitialised 4-bit matrix (a workspace, or the target of ``quantize_fp4_``)."""
+    """An uninitialised 4-bit matrix (the target of ``quantize_fp4_``)."""
     _check_format(format)
     if rows < 0 or cols < 1:
         raise ValueError(f"a 4-bit matrix has at least one column, got [{rows}, {cols}]")
-    per_chunk = 4 * FP4_BLOCK[format]
-    codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=device)
-    scales = torch.empty(((rows + 127) // 128, (cols + per_chunk - 1) // per_chunk, 512), dtype=torch.uint8,
-                         device=device)
-    return Fp4Tensor(codes, scales, rows, cols, format, _check_tensor_scale(format, tensor_scale))
+    scale = _check_tensor_scale(format, tensor_scale)
+    return Fp4Tensor._uninitialised(torch.empty(0, dtype=torch.uint8, device=device), rows, cols, format, scale)
 
 
 def fp4_tensor_scale(amax: float) -> float:
@@ -107,33 +145,41 @@ def _rows_to_write(out: torch.Tensor) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 def quantize_fp4_(out: Fp4Tensor, x: torch.Tensor) -> Fp4Tensor:
     """Quantise x [..., cols] BF16 into ``out`` (its format and tensor scale)."""
-    require_cuda(out.codes, out.scales, x)
+    require_cuda(out._buffer, x)
     x2 = _rows_of(x)
     if x2.shape != (out.rows, out.cols):
         raise ValueError(f"x has shape {tuple(x2.shape)}, the 4-bit matrix {out.shape}")
-    call("h3_quantize_fp4", desc(out.codes), desc(out.scales), desc(x2), _FORMAT[out.format], out.tensor_scale,
+    call("h3_quantize_fp4", out.d_codes, out.d_scales, packed(x2), _FORMAT[out.format], out.tensor_scale,
          stream_of(x))
     return out
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: float = 1.0) -> Fp4Tensor:
     """x [..., cols] BF16 as a 4-bit matrix of its rows."""
+    code = _check_format(format)
+    scale = _check_tensor_scale(format, tensor_scale)
+    require_cuda(x)
     x2 = _rows_of(x)
-    return quantize_fp4_(fp4_empty(x2.shape[0], x2.shape[1], format, tensor_scale, x.device), x2)
+    rows, cols = x2.shape
+    if cols < 1:
+        raise ValueError("a 4-bit matrix has at least one column")
+    out = Fp4Tensor._uninitialised(x, rows, cols, format, scale)
+    call("h3_quantize_fp4", out.d_codes, out.d_scales, packed(x2), code, scale, stream_of(x))
+    return out
 
 
 def dequantize_fp4_(out: torch.Tensor, q: Fp4Tensor) -> torch.Tensor:
-    require_cuda(out, q.codes, q.scales)
-    if tuple(out.shape) != q.shape:
+    require_cuda(out, q._buffer)
+    if out.shape != q.shape:
         raise ValueError(f"out has shape {tuple(out.shape)}, the 4-bit matrix {q.shape}")
-    call("h3_dequantize_fp4", desc(out), desc(q.codes), desc(q.scales), _FORMAT[q.format], q.tensor_scale,
+    call("h3_dequantize_fp4", packed(out), q.d_codes, q.d_scales, _FORMAT[q.format], q.tensor_scale,
          stream_of(out))
     return out
 
 
 def dequantize_fp4(q: Fp4Tensor) -> torch.Tensor:
     """The values a 4-bit matrix stands for, [rows, cols] BF16 (exact)."""
-    return dequantize_fp4_(torch.empty(q.rows, q.cols, dtype=torch.bfloat16, device=q.device), q)
+    return dequantize_fp4_(q._buffer.new_empty((q.rows, q.cols), dtype=torch.bfloat16), q)
 
 
 def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, format: str, cols: int | None = None,
@@ -189,33 +235,29 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
     several projections share it."""
     o2 = _rows_to_write(out)
     if isinstance(x, Fp4Tensor):
-        require_cuda(out, x.codes, x.scales, weight.codes, weight.scales, bias)
+        require_cuda(out, x._buffer, weight._buffer, bias)
         if x.format != weight.format:
             raise ValueError(f"x is {x.format}, the weight {weight.format}")
         if x.cols != weight.cols:
             raise ValueError(f"x has {x.cols} columns, the weight {weight.cols}")
-        call("h3_linear_fp4_quantized", desc(o2), desc(x.codes), desc(x.scales), desc(weight.codes),
-             desc(weight.scales), desc(bias), x.cols, _FORMAT[weight.format], x.tensor_scale, weight.tensor_scale,
-             stream_of(out))
+        call("h3_linear_fp4_quantized", packed(o2), x.d_codes, x.d_scales, weight.d_codes, weight.d_scales,
+             packed(bias), x.cols, _FORMAT[weight.format], x.tensor_scale, weight.tensor_scale, stream_of(out))
         return out
     x2 = _rows_of(x)
-    if x2.shape[1] != weight.cols:
-        raise ValueError(f"x has {x2.shape[1]} columns, the weight {weight.cols}")
-    require_cuda(out, x, weight.codes, weight.scales, bias)
+    rows, cols = x2.shape
+    if cols != weight.cols:
+        raise ValueError(f"x has {cols} columns, the weight {weight.cols}")
+    require_cuda(out, x, weight._buffer, bias)
     scale = _check_tensor_scale(weight.format, x_tensor_scale)
-    # x in 4 bits, codes then scales, in one allocation
-    rows, pitch = x2.shape[0], (weight.cols + 31) // 32 * 16
-    chunks_m, chunks_k = (rows + 127) // 128, weight.scales.shape[1]
-    work = torch.empty(rows * pitch + chunks_m * chunks_k * 512, dtype=torch.uint8, device=x.device)
-    at = work.data_ptr()
-    call("h3_linear_fp4", desc(o2), desc(x2), desc_rows(at, torch.uint8, rows, pitch),
-         desc_rows(at + rows * pitch, torch.uint8, chunks_m, chunks_k, 512), desc(weight.codes), desc(weight.scales),
-         desc(bias), _FORMAT[weight.format], scale, weight.tensor_scale, stream_of(x))
+    pitch, groups, chunks = _layout(rows, cols, weight.format)
+    work = x.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)   # x in 4 bits
+    call("h3_linear_fp4", packed(o2), packed(x2), packed(work), weight.d_codes, weight.d_scales, packed(bias),
+         _FORMAT[weight.format], scale, weight.tensor_scale, stream_of(x))
     return out
 
 
 def linear_fp4(x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
                x_tensor_scale: float = 1.0) -> torch.Tensor:
     lead = (x.rows,) if isinstance(x, Fp4Tensor) else x.shape[:-1]
-    out = torch.empty((*lead, weight.rows), dtype=torch.bfloat16, device=x.device)
+    out = weight._buffer.new_empty((*lead, weight.rows), dtype=torch.bfloat16)
     return linear_fp4_(out, x, weight, bias, x_tensor_scale)

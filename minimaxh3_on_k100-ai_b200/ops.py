@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import call, desc, require_cuda, stream_of
+from ._lib import call, desc, packed, require_cuda, stream_of
 
 __all__ = [
     "h3_rms_norm", "h3_rms_norm_", "h3_swiglu", "h3_swiglu_", "h3_rms_modulate", "h3_rms_modulate_",
@@ -199,12 +199,12 @@ def cross_attention_(out, q, k, v, lengths=None, scale=None):
         scale = q.shape[-1] ** -0.5
     if not 0.0 < scale <= 3e38:
         raise ValueError(f"the scale must be positive and finite, got {scale}")
-    call("h3_cross_attention", desc(out), desc(q), desc(k), desc(v), desc(lengths), scale, stream_of(q))
+    call("h3_cross_attention", packed(out), packed(q), packed(k), packed(v), packed(lengths), scale, stream_of(q))
     return out
 
 
 def cross_attention(q, k, v, lengths=None, scale=None):
-    return cross_attention_(torch.empty(q.shape, dtype=q.dtype, device=q.device), q, k, v, lengths, scale)
+    return cross_attention_(q.new_empty(q.shape), q, k, v, lengths, scale)
 
 
 # ---------------------------------------------------------------------------

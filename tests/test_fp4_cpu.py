@@ -87,10 +87,9 @@ def test_entry_points_refuse_bad_arguments(h3):
     bias = torch.zeros(4, dtype=torch.bfloat16)
     y = torch.zeros(4, 4, dtype=torch.bfloat16)
 
-    def linear(y, x, w, bias, fmt=1, tx=1.0):
+    def linear(y, x, w, bias, fmt=1, tx=1.0, work=torch.zeros(4 * 32 + 512, dtype=torch.uint8)):
         b = None if bias is None else ctypes.byref(d(bias))
-        return lib.h3_linear_fp4(*[ctypes.byref(d(a)) for a in (y, x, q.codes, q.scales, w.codes, w.scales)], b, fmt,
-                                 tx, 1.0, null)
+        return lib.h3_linear_fp4(*[ctypes.byref(d(a)) for a in (y, x, work, w.codes, w.scales)], b, fmt, tx, 1.0, null)
 
     assert linear(y.float(), x, q, None) == 3
     assert linear(torch.zeros(4, 5, dtype=torch.bfloat16), x, q, None) == 2
@@ -99,6 +98,8 @@ def test_entry_points_refuse_bad_arguments(h3):
     assert linear(y, x, q, bias.float()) == 3
     assert linear(y.t(), x, q, bias) == 4
     assert linear(y, x, q, bias, tx=0.3) == 5
+    assert linear(y, x, q, bias, work=torch.zeros(4 * 32 + 511, dtype=torch.uint8)) == 2    # a byte short
+    assert linear(y, x, q, bias, work=torch.zeros(1000, dtype=torch.bfloat16)) == 3
     empty = h3.fp4_empty(0, 48, "nvfp4", device="cpu")
     assert linear(torch.zeros(4, 0, dtype=torch.bfloat16), x, empty, None) == 0   # nothing to do
 
