@@ -20,8 +20,8 @@
 // it), O accumulated in fp32 and rounded once.
 //
 // rows form (a token, or a few, per sample): bound by reading K and V, so the keys are
-// split over the warps of a CTA and the CTAs of a cluster.  A producer warp streams 64-key
-// tiles by TMA through a ring; each of four warps takes 16 keys of a tile against all the
+// split over the warps of a CTA and the CTAs of a cluster.  A producer warp streams key
+// tiles by TMA through a ring; each computing warp takes 16 keys of a tile against all the
 // rows (mma.sync m16n8k16: the rows fill an M of 16 or 32, a 128-row tcgen05 tile would be
 // nearly empty and its softmax a single lane per row), with its own running maximum and
 // sum.  Partial results join in shared memory, then over the cluster through distributed
@@ -59,6 +59,7 @@ struct Params {
     float scale_log2;
     const int64_t *lens;         // [B] or null
     int items, per_head;         // tile form: work items, items per (sample, head)
+    int ordered;                 // samples with more states first
     // rows form: row r of a (sample, key/value head) is query r / group, head r % group of the group
     const __nv_bfloat16 *q;
     __nv_bfloat16 *out;
@@ -79,18 +80,23 @@ __device__ __forceinline__ int states(const Params &p, int b) {
 // ---------------------------------------------------------------------------
 constexpr int BM = 128, BN = 128;
 constexpr int TILE_THREADS = 384;
+constexpr int MAX_ORDERED = 512;                 // samples that are sorted by length; more are taken as they come
 
 template <int NQ>                                // Q tiles per work item: 1 or 2
 struct Tile {
-    static constexpr int KSLOTS = 2;
-    static constexpr int VSLOTS = NQ == 2 ? 1 : 2;   // a lone tile's softmax does not hide a V load
+    // S_t(j+1) is computed as soon as softmax t has read S_t(j), a whole step ahead of its
+    // use, so K_{j+1} may load after both S(j): one slot.  P_t(j+1) V_{j+1} comes right
+    // when its P is ready, so V_{j+1} has to be there by then: two.
+    static constexpr int KSLOTS = NQ == 2 ? 1 : 2;
+    static constexpr int VSLOTS = 2;
     static constexpr int OFF_Q = 0;
     static constexpr int OFF_P = OFF_Q + NQ * TILE_BYTES;
     static constexpr int OFF_K = OFF_P + NQ * TILE_BYTES;
     static constexpr int OFF_V = OFF_K + KSLOTS * TILE_BYTES;
     static constexpr int OFF_BAR = OFF_V + VSLOTS * TILE_BYTES;
     static constexpr int NUM_BARS = 2 * KSLOTS + 3 * VSLOTS + 6 * NQ;
-    static constexpr int SMEM = OFF_BAR + NUM_BARS * 8 + 16 + 1024;
+    static constexpr int OFF_ORDER = OFF_BAR + NUM_BARS * 8 + 16;
+    static constexpr int SMEM = OFF_ORDER + MAX_ORDERED * 2 + 1024;
     static constexpr uint32_t TMEM = NQ * 256;
     static constexpr int O_COL = NQ * BN;
     static_assert(SMEM <= 232448, "shared memory");
@@ -116,6 +122,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     uint64_t *o_done = p_ready + NQ;          // [t]: P_t(j) V_j has landed in O_t
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_done + NQ);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    uint16_t *order = reinterpret_cast<uint16_t *>(smem + C::OFF_ORDER);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -144,6 +151,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         tmem_alloc(tmem_slot, C::TMEM);
         tmem_relinquish();
     }
+    if (p.ordered) {
+        // samples by their number of key tiles, most first (their rank by counting)
+        int *cost = reinterpret_cast<int *>(smem + C::OFF_Q);
+        for (int i = threadIdx.x; i < p.B; i += TILE_THREADS) cost[i] = (states(p, i) + BN - 1) / BN;
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.B; i += TILE_THREADS) {
+            const int mine = cost[i];
+            int r = 0;
+            for (int j = 0; j < p.B; ++j) r += cost[j] > mine || (cost[j] == mine && j < i);
+            order[r] = (uint16_t)i;
+        }
+        fence_proxy_async_smem();   // Q's tile is loaded over the costs
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -151,11 +171,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 
     // Every role walks the same items; an item's number of key tiles comes from its
     // sample's length.  `n` counts key tiles over all items, `qi` items with any.
-    auto item_at = [&](int item, int &b, int &h, int &q0, int &len) {
+    auto item_at = [&](int i, int &b, int &h, int &q0, int &len) {
+        // round k deals items k G .. k G + G - 1 to the G CTAs, every other round in reverse:
+        // whoever got a long one gets a short one next
+        const int k = i / (int)gridDim.x, c = i - k * (int)gridDim.x;
+        const int item = p.ordered && (k & 1) ? min(p.items - k * (int)gridDim.x, (int)gridDim.x) - 1 - c + k * (int)gridDim.x : i;
         const int hb = item / p.per_head;
         b = hb / p.H;
         h = hb - b * p.H;
         q0 = (item - hb * p.per_head) * NQ * BM;
+        if (p.ordered) b = order[b];
         len = states(p, b);
     };
     bool ok = true;
@@ -457,24 +482,25 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 // ---------------------------------------------------------------------------
 // rows form
 // ---------------------------------------------------------------------------
-constexpr int KEYS = 64;                         // keys per tile: 16 for each of four warps
-constexpr int ROW_WARPS = 4;
-constexpr int ROW_THREADS = (ROW_WARPS + 1) * 32;
-constexpr int KV_BYTES = KEYS * HD * 2;          // a K or V tile
-constexpr int KV_HALF = KV_BYTES / 2;
+constexpr int KW = 16;                           // keys per warp and tile
+constexpr int MAX_SPLIT = 16;                    // CTAs per cluster
 
-template <int MT>                                // 16-row MMA tiles: rows per CTA / 16
+template <int MT, int WARPS>                     // 16-row MMA tiles (rows per CTA / 16), warps that compute
 struct Rows {
     static constexpr int ROWS = 16 * MT;
+    static constexpr int THREADS = (WARPS + 1) * 32;
+    static constexpr int KEYS = WARPS * KW;      // keys per tile
+    static constexpr int KV_BYTES = KEYS * HD * 2;   // a K or V tile
+    static constexpr int KV_HALF = KV_BYTES / 2;
     static constexpr int STAGES = 3;
     static constexpr int RING = STAGES * 2 * KV_BYTES;
     // in the ring's place at the end: O of each warp, then their sum (a float4 of padding
     // per row keeps the four lanes of a quad on different banks)
     static constexpr int PITCH = HD + 4;
-    static constexpr int OFF_SUM = ROW_WARPS * ROWS * PITCH * 4;
+    static constexpr int OFF_SUM = WARPS * ROWS * PITCH * 4;
     static constexpr int OFF_BAR = RING > OFF_SUM + ROWS * PITCH * 4 ? RING : OFF_SUM + ROWS * PITCH * 4;
-    static constexpr int OFF_ML = OFF_BAR + 2 * STAGES * 8 + 16;         // [warp 0..3, joint][row] maximum and sum
-    static constexpr int SMEM = OFF_ML + (ROW_WARPS + 1) * ROWS * 8 + 1024;
+    static constexpr int OFF_ML = OFF_BAR + 2 * STAGES * 8 + 16;         // [warp, joint][row] maximum and sum
+    static constexpr int SMEM = OFF_ML + (WARPS + 1) * ROWS * 8 + 1024;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -490,7 +516,7 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -515,10 +541,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
 }
 
 // grid: x = cluster rank (share of the keys), y = (sample, key/value head, row chunk)
-template <int MT>
-__global__ void __launch_bounds__(ROW_THREADS)
+template <int MT, int WARPS>
+__global__ void __launch_bounds__(Rows<MT, WARPS>::THREADS)
     rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, Params p) {
-    using C = Rows<MT>;
+    using C = Rows<MT, WARPS>;
+    constexpr int ROW_WARPS = WARPS, ROW_THREADS = C::THREADS, KEYS = C::KEYS, KV_BYTES = C::KV_BYTES, KV_HALF = C::KV_HALF;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
@@ -602,25 +629,35 @@ __global__ void __launch_bounds__(ROW_THREADS)
             const int s = i % C::STAGES;
             ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (i / C::STAGES) & 1, abort_flag));
             if (!ok) break;
-            const int key0 = (t0 + i) * KEYS + warp * 16;         // this warp's 16 keys
+            const int key0 = (t0 + i) * KEYS + warp * KW;         // this warp's KW keys
             if (key0 < len) {
                 const uint32_t kt = smem_u32(smem + s * 2 * KV_BYTES), vt = kt + KV_BYTES;
                 // lanes 0-7, 8-15, 16-23, 24-31 address the four 8 x 8 matrices: keys 0-7 and
                 // 8-15 (K: bit 4 of the lane, V: bit 3), columns 0-7 and 8-15 (the other bit)
-                const int kr = warp * 16 + (lane & 7) + (lane & 16 ? 8 : 0), kc = lane & 8 ? 1 : 0;
-                const int vr = warp * 16 + (lane & 7) + (lane & 8 ? 8 : 0), vc = lane & 16 ? 1 : 0;
+                const int kr = warp * KW + (lane & 7) + (lane & 16 ? 8 : 0), kc = lane & 8 ? 1 : 0;
+                const int vr = warp * KW + (lane & 7) + (lane & 8 ? 8 : 0), vc = lane & 16 ? 1 : 0;
+                // fragments are fetched ahead of the products that use them: all of a row tile's,
+                // or (MT = 2, where registers are short) four at a time
+                constexpr int AHEAD = MT == 1 ? 8 : 4;
                 float sc[MT][2][4] = {};
+                uint32_t bf[AHEAD][4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    uint32_t bk[4];
-                    ldsm4(kt + (k >> 2) * KV_HALF + swz(kr, (k & 3) * 2 + kc), bk);
+                for (int k0 = 0; k0 < 8; k0 += AHEAD) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        mma16816(sc[mt][0], qf[mt][k], bk[0], bk[1]);
-                        mma16816(sc[mt][1], qf[mt][k], bk[2], bk[3]);
-                    }
+                    for (int k = 0; k < AHEAD; ++k)
+                        ldsm4(kt + ((k0 + k) >> 2) * KV_HALF + swz(kr, ((k0 + k) & 3) * 2 + kc), bf[k]);
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816(sc[mt][0], qf[mt][k0 + k], bf[k][0], bf[k][1]);
+                            mma16816(sc[mt][1], qf[mt][k0 + k], bf[k][2], bf[k][3]);
+                        }
                 }
-                const int valid = len - key0;                     // of these 16 keys
+                // the first of V's fragments, to arrive behind the softmax
+#pragma unroll
+                for (int d = 0; d < AHEAD; ++d) ldsm4_trans(vt + (d >> 2) * KV_HALF + swz(vr, (d & 3) * 2 + vc), bf[d]);
+                const int valid = len - key0;                     // of these KW keys
                 uint32_t pf[MT][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
@@ -633,8 +670,8 @@ __global__ void __launch_bounds__(ROW_THREADS)
                         }
 #pragma unroll
                     for (int hi = 0; hi < 2; ++hi) {
-                        float mx = fmaxf(fmaxf(sc[mt][0][2 * hi], sc[mt][0][2 * hi + 1]),
-                                         fmaxf(sc[mt][1][2 * hi], sc[mt][1][2 * hi + 1]));
+                        float mx = max3f(fmaxf(sc[mt][0][2 * hi], sc[mt][0][2 * hi + 1]), sc[mt][1][2 * hi],
+                                         sc[mt][1][2 * hi + 1]);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                         if (mx > m[mt][hi]) {                     // the same in the row's four lanes
@@ -647,32 +684,34 @@ __global__ void __launch_bounds__(ROW_THREADS)
                         const float base = m[mt][hi] == -INFINITY ? 0.f : m[mt][hi];
                         float pr[4];
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) pr[2 * nt + e] = ex2(sc[mt][nt][2 * hi + e] - base);
+                        for (int e = 0; e < 4; ++e) pr[e] = ex2(sc[mt][e >> 1][2 * hi + (e & 1)] - base);
                         l[mt][hi] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
                         pf[mt][hi] = pack_bf16x2(pr[0], pr[1]);
                         pf[mt][hi + 2] = pack_bf16x2(pr[2], pr[3]);
                     }
                 }
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    uint32_t bv[4];
-                    ldsm4_trans(vt + (d >> 2) * KV_HALF + swz(vr, (d & 3) * 2 + vc), bv);
-                    if (valid < 16) {                             // zeros for the rows behind the last state
-                        const int k0 = (lane & 3) * 2;
+                for (int d0 = 0; d0 < 8; d0 += AHEAD) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = k0 + (e & 1) * 8;
-                            if (key >= valid) bv[e] = 0;
-                            else if (key + 1 >= valid) bv[e] &= 0xffffu;
+                    for (int d = 0; d < AHEAD && d0 > 0; ++d)
+                        ldsm4_trans(vt + ((d0 + d) >> 2) * KV_HALF + swz(vr, ((d0 + d) & 3) * 2 + vc), bf[d]);
+                    if (valid < KW) {                             // zeros for the rows behind the last state
+#pragma unroll
+                        for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = (lane & 3) * 2 + (e & 1) * 8;
+                                if (key >= valid) bf[d][e] = 0;
+                                else if (key + 1 >= valid) bf[d][e] &= 0xffffu;
+                            }
+                    }
+#pragma unroll
+                    for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816(o[mt][2 * (d0 + d)], pf[mt], bf[d][0], bf[d][1]);
+                            mma16816(o[mt][2 * (d0 + d) + 1], pf[mt], bf[d][2], bf[d][3]);
                         }
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        mma16816(o[mt][2 * d], pf[mt], bv[0], bv[1]);
-                        mma16816(o[mt][2 * d + 1], pf[mt], bv[2], bv[3]);
-                    }
                 }
             }
             __syncwarp();
@@ -701,7 +740,7 @@ __global__ void __launch_bounds__(ROW_THREADS)
                 }
             }
         named_bar_sync(1, ROW_WARPS * 32);
-        // the four warps' results as one
+        // the warps' results as one
         float *sum_o = o_part + ROW_WARPS * C::ROWS * C::PITCH;
         for (int i = threadIdx.x; i < rows * (HD / 4); i += ROW_WARPS * 32) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -734,29 +773,35 @@ __global__ void __launch_bounds__(ROW_THREADS)
         const uint32_t o_at = smem_u32(o_part + ROW_WARPS * C::ROWS * C::PITCH);
         for (int i = rank * ROW_THREADS + threadIdx.x; i < rows * (HD / 4); i += split * ROW_THREADS) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            float mr[8], lr[8];
-            float4 v[8];
+            float mr[MAX_SPLIT], top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (c < split) {
-                    mr[c] = ld_cluster_f32(m_at + r * 4, c);
-                    lr[c] = ld_cluster_f32(l_at + r * 4, c);
-                    v[c] = ld_cluster_f4(o_at + (r * C::PITCH + d) * 4, c);
-                }
-            float top = -INFINITY;
+            for (int c = 0; c < MAX_SPLIT; ++c)
+                if (c < split) mr[c] = ld_cluster_f32(m_at + r * 4, c);
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
+            for (int c = 0; c < MAX_SPLIT; ++c)
                 if (c < split) top = fmaxf(top, mr[c]);
             const float base = top == -INFINITY ? 0.f : top;
             float lt = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            // eight ranks' pieces are requested before the first is needed
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                if (c < split) {
-                    const float f = ex2(mr[c] - base);
-                    lt += lr[c] * f;
-                    acc.x += v[c].x * f, acc.y += v[c].y * f, acc.z += v[c].z * f, acc.w += v[c].w * f;
-                }
+            for (int c0 = 0; c0 < MAX_SPLIT; c0 += 8) {
+                float lr[8];
+                float4 v[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c0 + c < split) {
+                        lr[c] = ld_cluster_f32(l_at + r * 4, c0 + c);
+                        v[c] = ld_cluster_f4(o_at + (r * C::PITCH + d) * 4, c0 + c);
+                    }
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c0 + c < split) {
+                        const float f = ex2(mr[c0 + c] - base);
+                        lt += lr[c] * f;
+                        acc.x += v[c].x * f, acc.y += v[c].y * f, acc.z += v[c].z * f, acc.w += v[c].w * f;
+                    }
+            }
             const float inv = lt == 0.f ? 0.f : 1.0f / lt;        // no state, or none with a finite score
             const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
             *reinterpret_cast<uint2 *>(p.out + row_at(r, p.o_b, p.o_s, p.o_h) + d) = pack4(f);
@@ -831,59 +876,112 @@ int launch_tiles(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, c
     if (items > 0x3fffffff) return H3_ERR_UNSUPPORTED;
     p.items = (int)items;
     const int grid = p.items < num_sms() ? p.items : num_sms();
+    // with a length per sample items differ in cost: dealt in descending order they level out
+    p.ordered = p.lens && p.B > 1 && p.B <= cross::MAX_ORDERED && p.items > grid;
     cross::tile_kernel<NQ><<<grid, cross::TILE_THREADS, C::SMEM, stream>>>(tq, tk, tv, to, p);
     return launch_status();
 }
 
-template <int MT>
+template <int MT, int WARPS>
+void rows_config(cudaLaunchConfig_t *cfg, cudaLaunchAttribute *attr) {
+    using C = cross::Rows<MT, WARPS>;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = 1;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cfg->blockDim = dim3(C::THREADS);
+    cfg->dynamicSmemBytes = C::SMEM;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
+}
+
+// In how many shares the keys of `groups` (sample, key/value head, row chunk) groups are
+// taken: as many as run in one wave and have a key tile each.  0: the device cannot say.
+template <int MT, int WARPS>
+int rows_split(int64_t groups, int Sk) {
+    using C = cross::Rows<MT, WARPS>;
+    auto kernel = cross::rows_kernel<MT, WARPS>;
+    // per device: clusters of 1..16 CTAs resident at once (a cluster stays within one group
+    // of SMs, so large ones leave SMs empty: 148 SMs hold 15 clusters of 8 one-CTA SMs)
+    static std::atomic<int> resident[64][cross::MAX_SPLIT + 1];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 0;
+    if (resident[dev][1].load() == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        rows_config<MT, WARPS>(&cfg, &attr);
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return 0;
+        for (int c = cross::MAX_SPLIT; c >= 1; --c) {
+            attr.val.clusterDim.x = c;
+            cfg.gridDim = dim3(c, 1024, 1);
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+            resident[dev][c].store(n);
+        }
+        if (resident[dev][1].load() < 1) return 0;
+    }
+    const int tiles = (Sk + C::KEYS - 1) / C::KEYS;
+    int split = tiles < 1 ? 1 : tiles < cross::MAX_SPLIT ? tiles : cross::MAX_SPLIT;
+    while (split > 1 && resident[dev][split].load() < groups) --split;
+    return split;
+}
+
+template <int MT, int WARPS>
 int launch_rows(const h3_tensor *k, const h3_tensor *v, cross::Params &p, cudaStream_t stream) {
-    using C = cross::Rows<MT>;
-    auto kernel = cross::rows_kernel<MT>;
+    using C = cross::Rows<MT, WARPS>;
     CUtensorMap tk{}, tv{};
     if (p.Sk > 0) {
-        H3_CHECK(heads_tmap(&tk, k, p.kv_shared ? 1 : p.B, cross::KEYS));
-        H3_CHECK(heads_tmap(&tv, v, p.kv_shared ? 1 : p.B, cross::KEYS));
+        H3_CHECK(heads_tmap(&tk, k, p.kv_shared ? 1 : p.B, C::KEYS));
+        H3_CHECK(heads_tmap(&tv, v, p.kv_shared ? 1 : p.B, C::KEYS));
     }
     p.chunks = (p.rows + C::ROWS - 1) / C::ROWS;
     const int64_t groups = (int64_t)(p.fold ? 1 : p.B) * p.kv_heads * p.chunks;
     if (groups > 65535) return H3_ERR_UNSUPPORTED;
+    const int split = rows_split<MT, WARPS>(groups, p.Sk);
+    if (split < 1) return H3_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(cross::ROW_THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    static std::atomic<int> resident[64][9];   // per device: clusters of 1..8 CTAs resident at once
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
-    if (resident[dev][1].load() == 0) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-            return H3_ERR_LAUNCH;
-        for (int c = 8; c >= 1; --c) {
-            attr[0].val.clusterDim.x = c;
-            cfg.gridDim = dim3(c, 1024, 1);
-            int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return H3_ERR_LAUNCH;
-            resident[dev][c].store(n);
-        }
-    }
-    // key shares: as many as run in one wave and have a tile each
-    const int tiles = (p.Sk + cross::KEYS - 1) / cross::KEYS;
-    int split = tiles < 1 ? 1 : tiles < 8 ? tiles : 8;
-    while (split > 1 && resident[dev][split].load() < groups) --split;
-    attr[0].val.clusterDim.x = split;
+    cudaLaunchAttribute attr;
+    rows_config<MT, WARPS>(&cfg, &attr);
+    attr.val.clusterDim.x = split;
     cfg.gridDim = dim3(split, (unsigned)groups, 1);
-    if (cudaLaunchKernelEx(&cfg, kernel, tk, tv, p) != cudaSuccess) {
+    cfg.stream = stream;
+    if (cudaLaunchKernelEx(&cfg, cross::rows_kernel<MT, WARPS>, tk, tv, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;
     }
     return launch_status();
+}
+
+// Whether the rows form takes less time than the tile form, from the times of one step of
+// either measured on B200 (us): a key tile of the rows form 1.05 (16 rows, 128 keys, one
+// CTA per SM), 1.45 (16 rows, 64 keys, two) or 1.1 (32 rows, 64 keys); 128 keys of one Q tile
+// 1.47, of two 2.07, and 1.5 to store an item; the rest of a launch 5 to 9.5.  Checked at
+// 16..512 queries, 512..18432 states, 2..640 groups: e.g. 32 queries, 40 heads, 512 states
+// 13.0 us in rows and 11.3 in tiles, 2304 states 22.5 and 29.7; 512 queries of 2 heads over
+// 18432 states 79 and 197.
+bool rows_form(const cross::Params &p, int64_t rows, int64_t groups) {
+    const int sms = num_sms();
+    const int64_t tiles = (p.Sq + cross::BM - 1) / cross::BM, heads = (int64_t)p.H * p.B;
+    const double nkv = (p.Sk + 127) / 128;
+    const bool two = tiles > 1 && tiles * heads > sms;
+    const int64_t items = two ? (tiles + 1) / 2 * heads : tiles * heads;
+    const double waves = (double)((items + sms - 1) / sms);
+    const double in_tiles = 5.0 + waves * (nkv * (two ? 2.07 : 1.47) + 1.5);
+    double in_rows;
+    if (rows <= 16) {
+        in_rows = groups <= sms ? 6.0 + (nkv / (rows_split<1, 8>(groups, p.Sk) + 1e-9) + 0.5) * 1.05
+                                : 6.0 + (double)((groups + 2 * sms - 1) / (2 * sms)) * 2 * nkv * 1.45;
+    } else {
+        const double per = 2 * nkv / (rows_split<2, 4>(groups, p.Sk) + 1e-9) + 0.5;
+        in_rows = 9.5 + (double)((groups + sms - 1) / sms) * per * 1.1;
+    }
+    return in_rows < in_tiles;
 }
 
 }  // namespace
@@ -932,12 +1030,16 @@ extern "C" int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, cons
     p.fold = p.kv_shared && !p.lens;
     const int64_t rows = (int64_t)p.Sq * p.group * (p.fold ? B : 1);
     const int variant = g_variant.load();
-    const int64_t chunks = (rows + 31) / 32;
-    const bool fits = (p.fold ? 1 : B) * Hkv * chunks <= 65535 && rows <= 0x3fffffff;
-    if (variant == 1 ? fits : (variant == 0 && rows <= 32 && fits)) {
+    const int64_t groups = (p.fold ? 1 : B) * Hkv * (rows <= 16 ? 1 : (rows + 31) / 32);
+    const bool fits = groups <= 65535 && rows <= 0x3fffffff;
+    if (fits && (variant == 1 || (variant == 0 && rows_form(p, rows, groups)))) {
         p.rows = (int)rows;
-        return rows <= 16 ? launch_rows<1>(k, v, p, (cudaStream_t)stream)
-                          : launch_rows<2>(k, v, p, (cudaStream_t)stream);
+        if (rows > 16) return launch_rows<2, 4>(k, v, p, (cudaStream_t)stream);
+        // Eight warps fill an SM on their own, four leave room for a second CTA.  Measured at one
+        // query, 18432 states, 8 key/value heads (cluster of 16): 18.8 us with eight, 21.6 with four;
+        // at 160 (sample, head) groups of 512 states, more than there are SMs: 16.0 and 11.7 us.
+        return groups <= num_sms() ? launch_rows<1, 8>(k, v, p, (cudaStream_t)stream)
+                                   : launch_rows<1, 4>(k, v, p, (cudaStream_t)stream);
     }
     // one Q tile per item where that leaves no SM more than its share, two otherwise
     const int64_t tiles = (int64_t)(p.Sq + cross::BM - 1) / cross::BM;
