@@ -337,7 +337,9 @@ int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tenso
 /* y [M,N] = bf16(xq wq^T + bias): x [M,K] BF16 is quantised into the workspace (U8, 1-D,
  * 16-byte aligned, any contents, at least as many bytes as x's codes and scales together)
  * and multiplied with the 4-bit weight [N,K] of the same format; fp32 accumulation, one
- * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1. */
+ * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1.
+ * With a NULL workspace (at most 8 rows) the product quantises x itself, in one launch;
+ * the results are those of form 1 of h3_fp4_variant. */
 int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace, const h3_tensor *w_codes,
                   const h3_tensor *w_scales, const h3_tensor *bias, int32_t format, float x_tensor_scale,
                   float w_tensor_scale, void *stream);

@@ -139,11 +139,12 @@ def packed(t: torch.Tensor | None) -> bytes | None:
     """``desc`` as bytes, for the entry points that take ``D`` arguments (0.3 us less each)."""
     if t is None:
         return None
-    n = t.dim()
+    shape = t.shape
+    n = len(shape)
     code = _DTYPES.get(t.dtype)
     if n > 4 or code is None:
         desc(t)   # raises
-    return _PACK[n](t.data_ptr(), *t.shape, *t.stride(), n, code)
+    return _PACK[n](t.data_ptr(), *shape, *t.stride(), n, code)
 
 
 def packed_bytes(ptr: int, shape: tuple, strides: tuple) -> bytes:
@@ -191,17 +192,18 @@ def check_device(where: str) -> None:
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:
-    dev = -1
+    dev = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()     # -1 on the CPU
+        if dev is None:
+            dev = d
+        if d < 0 or not t.is_cuda:
             raise ValueError("H3 ops take CUDA tensors only (no CPU fallback)")
-        if dev < 0:
-            dev = t.get_device()
-        elif t.get_device() != dev:
+        if d != dev:
             raise ValueError("all tensors must be on the same device")
-    if dev >= 0 and dev != torch.cuda.current_device():
+    if dev is not None and dev != torch.cuda.current_device():
         raise ValueError(f"tensors on cuda:{dev} but the current device is cuda:{torch.cuda.current_device()}; "
                          "call under torch.cuda.device(...)")
 

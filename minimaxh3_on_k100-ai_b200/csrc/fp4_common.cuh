@@ -14,9 +14,12 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_fp16.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "h3_abi_util.h"
+#include "h3_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace h3 {
@@ -56,6 +59,100 @@ inline bool tensor_scale_ok(int fmt, float t) {
     memcpy(&u, &t, 4);
     if (fmt == MX) return u == 0x3f800000u;
     return (u & 0x807fffffu) == 0 && t >= 0x1p-64f && t <= 0x1p64f;
+}
+
+// ---------------------------------------------------------------------------
+// quantisation of 16 columns by one thread
+// ---------------------------------------------------------------------------
+constexpr int UNIT = 16;
+
+// 16 columns of a row as packed BF16 pairs, zeros past the end
+template <bool VEC>
+__device__ __forceinline__ void load_unit(const __nv_bfloat16 *row, int col, int cols, uint32_t (&w)[8]) {
+    if (VEC && col + UNIT <= cols) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + col));
+        const uint4 b = __ldg(reinterpret_cast<const uint4 *>(row + col) + 1);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+    } else {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t lo = col + 2 * i < cols ? __ldg(p + col + 2 * i) : 0;
+            const uint32_t hi = col + 2 * i + 1 < cols ? __ldg(p + col + 2 * i + 1) : 0;
+            w[i] = lo | (hi << 16);
+        }
+    }
+}
+
+// two e2m1 codes: `lo` in the low nibble
+__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
+        : "=r"(r)
+        : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3(float v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+    return r & 0xffu;
+}
+__device__ __forceinline__ float from_e4m3(uint32_t b) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)b));
+    return __half2float(__ushort_as_half((unsigned short)(h & 0xffff)));
+}
+
+// Codes (8 bytes) and scale byte of a unit; an mxfp4 block is this lane's unit and its
+// neighbour's (lane ^ 1), so all lanes of the warp take part.
+template <int FMT>
+__device__ __forceinline__ void quantize_unit(const uint32_t (&w)[8], float tensor_scale, uint32_t (&c)[2],
+                                              uint32_t &byte) {
+    // magnitudes order as integers; at 0x7f80 and above they are infinite or NaN
+    uint32_t top2 = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top2 = __vmaxu2(top2, w[i] & 0x7fff7fffu);
+    uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+    if (FMT == MX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const bool bad = top >= 0x7f80u;
+    c[0] = c[1] = 0;
+    if (FMT == MX) {
+        // the exponent field of amax is floor(log2 amax) + 127 (0 below the normals)
+        const int e = (int)(top >> 7) - 2;
+        byte = bad ? 255u : (uint32_t)max(e, 0);
+        const float inv = __uint_as_float((254u - byte) << 23);      // 2^(127 - byte), exact
+        if (!bad) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i >> 2] |= e2m1x2(blo(w[i]) * inv, bhi(w[i]) * inv) << (8 * (i & 3));
+        }
+    } else {
+        const float amax = __uint_as_float(top << 16);
+        byte = bad ? 127u : e4m3(__fdiv_rn(amax, 6.0f * tensor_scale));
+        if (!bad && byte != 0) {
+            // x / scale lies on a border between two codes, a multiple of 1/4, or (x has 8
+            // significant bits, the scale 4) at least 1/300 of it away.  Adding and taking
+            // away 1.5 * 2^11 rounds the product with the reciprocal to a multiple of 2^-12,
+            // which puts the first kind exactly on its border and moves none across.
+            const float r = __frcp_rn(from_e4m3(byte) * tensor_scale);
+            constexpr float SNAP = 1.5f * 2048.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                c[i >> 2] |= e2m1x2(__fadd_rn(__fmaf_rn(blo(w[i]), r, SNAP), -SNAP),
+                                    __fadd_rn(__fmaf_rn(bhi(w[i]), r, SNAP), -SNAP))
+                             << (8 * (i & 3));
+        }
+    }
+}
+
+// The four scales of a chunk's word, gathered from the 4 (nvfp4) or 8 (mxfp4, each twice)
+// lanes that hold them; valid in the first of those.
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_word(uint32_t byte) {
+    constexpr int STEP = FMT == MX ? 2 : 1;
+    uint32_t word = byte | (__shfl_down_sync(0xffffffffu, byte, STEP) << 8);
+    return word | __shfl_down_sync(0xffffffffu, word, 2 * STEP) << 16;
 }
 
 }  // namespace fp4

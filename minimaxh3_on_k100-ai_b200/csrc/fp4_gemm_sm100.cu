@@ -12,6 +12,10 @@
 // sums its share of the columns over the cluster in rank order (fixed order, no atomics,
 // no scratch in global memory).  Bound by reading the weights (HBM).
 //
+// For up to 8 rows the same kernel can quantise x itself: four more warps write this CTA's
+// share of x to the ring, which saves a launch and the scratch (1 x 15360 x 5120 nvfp4:
+// 13.7 us against 14.3; 16 rows would take 12.9 against 9.6 at 5120 x 5120).
+//
 // tile form: persistent CTA pairs (cta_group::2), 256 x 256 output tiles, K in tiles of 256
 // (one 128-byte swizzle span of codes) through a 5-slot TMA ring.  Each CTA loads its 128 x
 // rows, half the tile's w rows, and the scales of its x rows and of all the w rows; the
@@ -50,6 +54,11 @@ struct Params {
     int num_m, num_n;            // tiles
     int wide;                    // 4-column (8-byte) stores allowed
     int dependent;               // launched behind the quantisation of x: only w may be read before it ends
+    // fused quantisation: x itself
+    const __nv_bfloat16 *x;
+    int64_t ldx;
+    int cols, x_vec;             // x_vec: 16-byte loads of x allowed
+    float x_scale;               // its tensor scale
 };
 
 template <int FMT, int BN>
@@ -72,6 +81,8 @@ struct Swap {
     static_assert(STAGES >= 3, "ring");
 };
 constexpr int SWAP_THREADS = 128;
+constexpr int QUANT_WARPS = 4;                   // of the fused form
+constexpr int FUSED_TILE = 16, FUSED_ROWS = 8;   // of the fused form: x tile, and how many rows it takes
 
 // 16 bytes from CTA `rank`'s shared memory at this CTA's address `addr`
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
@@ -98,8 +109,8 @@ __device__ __forceinline__ void st_shared_f32(uint32_t addr, uint32_t v) {
 }
 
 // grid: x = cluster rank (K share), y = weight row tile, z = x row tile
-template <int FMT, int BN>
-__global__ void __launch_bounds__(SWAP_THREADS)
+template <int FMT, int BN, bool FUSED>
+__global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0), 2)
     swap_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, Params p) {
     using C = Swap<FMT, BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -116,16 +127,33 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     const int k_begin = (int)((int64_t)p.ktiles * rank / split), k_end = (int)((int64_t)p.ktiles * (rank + 1) / split);
     const int nk = k_end - k_begin;
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+    auto load_w = [&](int i) {
+        const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
+        uint8_t *st = smem + slot * C::STAGE_PAD;
+        if (elect_one()) {
+            mbar_expect_tx(&full[slot], C::A_BYTES + ch * CHUNK + (FUSED ? 0 : C::B_BYTES + ch * CHUNK));
+            tma_load_2d(st, &tw, &full[slot], kt * 128, n0);
+            bulk_load(st + C::A_BYTES + C::B_BYTES, p.sw + ((int64_t)blockIdx.y * p.chunks + kt * C::CH) * CHUNK,
+                      ch * CHUNK, &full[slot]);
         }
-        mbar_init(done, 1);
-        *abort_flag = 0;
-        fence_mbar_init();
-    }
-    if (warp == 1) {
+        __syncwarp();
+    };
+    // the weights wait for nothing: warp 0 fills the ring with them before the rest is set up
+    const int head = min(nk, C::STAGES);
+    if (warp == 0) {
+        if (elect_one()) {
+            for (int s = 0; s < C::STAGES; ++s) {
+                mbar_init(&full[s], FUSED ? 2 : 1);
+                mbar_init(&empty[s], 1);
+            }
+            mbar_init(done, 1);
+            *abort_flag = 0;
+            fence_mbar_init();
+            fence_proxy_async_smem();   // the copies below come before any block barrier
+        }
+        __syncwarp();
+        for (int i = 0; i < head; ++i) load_w(i);
+    } else if (warp == 1) {
         tmem_alloc(tmem_slot, C::TMEM);
         tmem_relinquish();
     }
@@ -135,20 +163,10 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        auto load_w = [&](int i) {
-            const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
-            uint8_t *st = smem + slot * C::STAGE_PAD;
-            if (elect_one()) {
-                mbar_expect_tx(&full[slot], C::A_BYTES + C::B_BYTES + 2 * ch * CHUNK);
-                tma_load_2d(st, &tw, &full[slot], kt * 128, n0);
-                bulk_load(st + C::A_BYTES + C::B_BYTES, p.sw + ((int64_t)blockIdx.y * p.chunks + kt * C::CH) * CHUNK,
-                          ch * CHUNK, &full[slot]);
-            }
-            __syncwarp();
-        };
         auto load_x = [&](int i) {
             const int slot = i % C::STAGES, kt = k_begin + i, ch = min(C::CH, p.chunks - kt * C::CH);
             uint8_t *st = smem + slot * C::STAGE_PAD;
+            if (FUSED) return;
             if (elect_one()) {
                 tma_load_2d(st + C::A_BYTES, &tx, &full[slot], kt * 128, m0);
                 bulk_load(st + C::A_BYTES + C::B_BYTES + C::SF_BYTES,
@@ -156,9 +174,6 @@ __global__ void __launch_bounds__(SWAP_THREADS)
             }
             __syncwarp();
         };
-        // the weights do not wait for the quantisation of x: fill the ring with them first
-        const int head = min(nk, C::STAGES);
-        for (int i = 0; i < head; ++i) load_w(i);
         if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int i = 0; i < head; ++i) load_x(i);
         for (int i = head; i < nk; ++i) {
@@ -206,6 +221,62 @@ __global__ void __launch_bounds__(SWAP_THREADS)
             __syncwarp();
         }
         if (!ok) drain_in_flight();
+    } else if (FUSED && warp >= 4) {
+        // This CTA's share of x in 4 bits, straight to the ring.  A warp takes every fourth K
+        // tile whole, 16 lanes to a row; its next tile's columns load while it stores this
+        // one's.  Every CTA of a column of tiles repeats this, so it is for a few rows: then
+        // it costs less than a launch.
+        constexpr int PER = FUSED_ROWS / 2;                  // pairs of rows
+        const int half = lane >> 4, unit = lane & 15;
+        uint32_t w[PER][8];
+        auto load = [&](int i) {
+            const int col = (k_begin + i) * BK + unit * UNIT;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int r = 2 * j + half;
+                if (2 * j >= p.M) break;
+                if (r < p.M) {
+                    const __nv_bfloat16 *row = p.x + (int64_t)r * p.ldx;
+                    if (p.x_vec) load_unit<true>(row, col, p.cols, w[j]);
+                    else load_unit<false>(row, col, p.cols, w[j]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[j][e] = 0;
+                }
+            }
+        };
+        const int first = warp - 4;
+        if (first < nk) load(first);
+        for (int i = first; i < nk; i += QUANT_WARPS) {
+            const int slot = i % C::STAGES;
+            uint32_t c[PER][2], word[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (2 * j >= p.M) break;                     // uniform
+                uint32_t byte;
+                quantize_unit<FMT>(w[j], p.x_scale, c[j], byte);
+                word[j] = scale_word<FMT>(byte);
+            }
+            if (i + QUANT_WARPS < nk) load(i + QUANT_WARPS);
+            if (i >= C::STAGES &&
+                !__all_sync(0xffffffffu, mbar_wait(&empty[slot], (i / C::STAGES - 1) & 1, abort_flag)))
+                break;
+            const uint32_t sx = smem_u32(smem) + slot * C::STAGE_PAD + C::A_BYTES, ssx = sx + C::B_BYTES + C::SF_BYTES;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (2 * j >= p.M) break;
+                const int r = 2 * j + half;
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(sx + r * 128 + (((unit >> 1) ^ (r & 7)) << 4) +
+                                                                      (unit & 1) * 8),
+                             "r"(c[j][0]), "r"(c[j][1])
+                             : "memory");
+                constexpr int LANES = FMT == MX ? 8 : 4;     // units of a chunk
+                if (unit % LANES == 0) st_shared_f32(ssx + unit / LANES * CHUNK + r * 16, word[j]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[slot]);
+        }
     }
     __syncwarp();
     const bool ok = nk == 0 || __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag));
@@ -213,7 +284,7 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     // lane = weight row: column c of the tile becomes 128 consecutive floats
     const uint32_t red = smem_u32(smem);
     const int cols = min(BN, p.M - m0);
-    if (ok) {
+    if (ok && warp < 4) {
 #pragma unroll 1
         for (int c0 = 0; c0 < cols; c0 += 16) {
             uint32_t v[16];
@@ -229,7 +300,7 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     tc_fence_before();
     if (split > 1) cluster_sync();
     else __syncthreads();
-    if (ok) {
+    if (ok && warp < 4) {
         const int n = n0 + lane * 4;
         float b[4] = {0.f, 0.f, 0.f, 0.f};
         if (p.bias) {
@@ -268,56 +339,77 @@ __global__ void __launch_bounds__(SWAP_THREADS)
     }
 }
 
+// K shares of `tiles` output tiles: as many as run in one wave and have a K tile each, the
+// same for a fused product and for one of rows quantised beforehand.  0: cannot be told.
 template <int FMT, int BN>
-int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+int swap_split(int64_t tiles, int ktiles) {
     using C = Swap<FMT, BN>;
-    auto kernel = swap_kernel<FMT, BN>;
-    CUtensorMap tx, tw;
-    H3_CHECK(make_tmap_bytes(&tx, xc->data, xc->shape[1], xc->shape[0],
-                             xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, BN));
-    H3_CHECK(make_tmap_bytes(&tw, wc->data, wc->shape[1], wc->shape[0],
-                             wc->shape[0] > 1 ? wc->strides[0] : wc->shape[1], 128, 128));
-    p.num_m = (p.M + BN - 1) / BN;
-    p.num_n = (p.N + 127) / 128;
-    if (p.num_m > 65535 || p.num_n > 65535) return H3_ERR_UNSUPPORTED;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.blockDim = dim3(SWAP_THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     // Per device: how many clusters of 1..8 CTAs are resident at once.  A cluster stays
     // within one group of SMs, so 8-CTA clusters fill fewer SMs than their number suggests.
     static std::atomic<int> resident[64][9];
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
+    if (dev < 0 || dev >= 64) return 0;
     if (resident[dev][1].load() == 0) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-            return H3_ERR_LAUNCH;
+        auto plain = swap_kernel<FMT, BN, false>;
+        if (cudaFuncSetAttribute(plain, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return 0;
+        if constexpr (BN == FUSED_TILE) {
+            auto fused = swap_kernel<FMT, BN, true>;
+            if (cudaFuncSetAttribute(fused, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+                return 0;
+        }
         for (int c = 8; c >= 1; --c) {
-            attr[0].val.clusterDim.x = c;
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = c;
+            attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = 1;
             cfg.gridDim = dim3(c, 1024, 1);
+            cfg.blockDim = dim3(SWAP_THREADS);
+            cfg.dynamicSmemBytes = C::SMEM;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
             int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return H3_ERR_LAUNCH;
+            if (cudaOccupancyMaxActiveClusters(&n, plain, &cfg) != cudaSuccess || n < 1) return 0;
             resident[dev][c].store(n);
         }
     }
-    // K shares: as many as run in one wave
-    const int64_t tiles = (int64_t)p.num_m * p.num_n;
-    int split = p.ktiles < 8 ? p.ktiles : 8;
+    int split = ktiles < 8 ? ktiles : 8;
     while (split > 1 && resident[dev][split].load() < tiles) --split;
+    return split;
+}
+
+template <int FMT, int BN, bool FUSED>
+int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    using C = Swap<FMT, BN>;
+    CUtensorMap tx, tw;
+    H3_CHECK(make_tmap_bytes(&tw, wc->data, wc->shape[1], wc->shape[0],
+                             wc->shape[0] > 1 ? wc->strides[0] : wc->shape[1], 128, 128));
+    if (FUSED) tx = tw;   // not used
+    else
+        H3_CHECK(make_tmap_bytes(&tx, xc->data, xc->shape[1], xc->shape[0],
+                                 xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, BN));
+    p.num_m = (p.M + BN - 1) / BN;
+    p.num_n = (p.N + 127) / 128;
+    if (p.num_m > 65535 || p.num_n > 65535) return H3_ERR_UNSUPPORTED;
+    const int split = swap_split<FMT, BN>((int64_t)p.num_m * p.num_n, p.ktiles);
+    if (split < 1) return H3_ERR_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(split, p.num_n, p.num_m);
+    cfg.blockDim = dim3(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0));
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = attr;
     cfg.numAttrs = p.dependent ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, swap_kernel<FMT, BN, FUSED>, tx, tw, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;
     }
@@ -657,10 +749,16 @@ template <int FMT>
 int multiply(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
     const int v = g_variant.load();
     if (v == 2 || (v == 0 && p.M > 128)) return launch_tiles<FMT>(xc, wc, p, stream);
-    if (p.M <= 16) return launch_swap<FMT, 16>(xc, wc, p, stream);
-    if (p.M <= 32) return launch_swap<FMT, 32>(xc, wc, p, stream);
-    if (p.M <= 64) return launch_swap<FMT, 64>(xc, wc, p, stream);
-    return launch_swap<FMT, 128>(xc, wc, p, stream);
+    if (p.M <= 16) return launch_swap<FMT, 16, false>(xc, wc, p, stream);
+    if (p.M <= 32) return launch_swap<FMT, 32, false>(xc, wc, p, stream);
+    if (p.M <= 64) return launch_swap<FMT, 64, false>(xc, wc, p, stream);
+    return launch_swap<FMT, 128, false>(xc, wc, p, stream);
+}
+
+// x quantised inside the product (at most FUSED_ROWS rows)
+template <int FMT>
+int multiply_fused(const h3_tensor *wc, Params &p, cudaStream_t stream) {
+    return launch_swap<FMT, FUSED_TILE, true>(nullptr, wc, p, stream);
 }
 
 // Checks of y, bias and the operands' widths; fills everything but the tile counts.
@@ -725,23 +823,42 @@ extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_te
                              const h3_tensor *w_codes, const h3_tensor *w_scales, const h3_tensor *bias, int32_t format,
                              float x_tensor_scale, float w_tensor_scale, void *stream) {
     H3_CHECK(check_bf16(x));
-    H3_CHECK(check_desc(workspace, H3_U8));
     if (x->ndim != 2 || x->shape[1] < 1) return H3_ERR_BAD_SHAPE;
     if (format != fp4::MX && format != fp4::NV) return H3_ERR_UNSUPPORTED;
     const int64_t rows = x->shape[0], cols = x->shape[1];
     if (rows > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
+    if ((cols > 1 && x->strides[1] != 1) || (rows > 1 && x->strides[0] < 0)) return H3_ERR_BAD_LAYOUT;
     // x in 4 bits: its codes, then its scales
     const int64_t pitch = fp4::code_pitch(cols), groups = (rows + 127) / 128, chunks = fp4::scale_chunks(format, cols);
-    if (workspace->ndim != 1 || workspace->shape[0] < rows * pitch + groups * chunks * fp4::CHUNK)
-        return H3_ERR_BAD_SHAPE;
-    if (rows > 0 && (workspace->strides[0] != 1 || !aligned16(workspace->data))) return H3_ERR_BAD_LAYOUT;
-    uint8_t *at = static_cast<uint8_t *>(workspace->data);
-    const h3_tensor xc = {at, {rows, pitch}, {pitch, 1}, 2, H3_U8};
-    const h3_tensor xs = {at + rows * pitch, {groups, chunks, fp4::CHUNK}, {chunks * fp4::CHUNK, fp4::CHUNK, 1}, 3, H3_U8};
+    const bool fused = !workspace;
+    uint8_t *at = nullptr;
+    if (fused) {
+        if (rows > fp4::FUSED_ROWS) return H3_ERR_NULL;
+    } else {
+        H3_CHECK(check_desc(workspace, H3_U8));
+        if (workspace->ndim != 1 || workspace->shape[0] < rows * pitch + groups * chunks * fp4::CHUNK)
+            return H3_ERR_BAD_SHAPE;
+        if (rows > 0 && (workspace->strides[0] != 1 || !aligned16(workspace->data))) return H3_ERR_BAD_LAYOUT;
+        at = static_cast<uint8_t *>(workspace->data);
+    }
+    // (of a fused product only the shapes are looked at; its data pointers stand for themselves)
+    uint8_t *held = fused ? reinterpret_cast<uint8_t *>(uintptr_t(16)) : at;
+    const h3_tensor xc = {held, {rows, pitch}, {pitch, 1}, 2, H3_U8};
+    const h3_tensor xs = {held + rows * pitch, {groups, chunks, fp4::CHUNK}, {chunks * fp4::CHUNK, fp4::CHUNK, 1}, 3, H3_U8};
     fp4::Params p{};
     H3_CHECK(fp4::check_product(y, &xc, &xs, w_codes, w_scales, bias, rows, cols, format, x_tensor_scale,
                                 w_tensor_scale, &p));
     if (p.M == 0 || p.N == 0) return H3_OK;
+    if (fused) {
+        p.sx = nullptr;
+        p.x = static_cast<const __nv_bfloat16 *>(x->data);
+        p.ldx = rows > 1 ? x->strides[0] : 0;
+        p.cols = (int)cols;
+        p.x_vec = aligned16(x->data) && p.ldx % 8 == 0;
+        p.x_scale = x_tensor_scale;
+        return format == fp4::MX ? fp4::multiply_fused<fp4::MX>(w_codes, p, (cudaStream_t)stream)
+                                 : fp4::multiply_fused<fp4::NV>(w_codes, p, (cudaStream_t)stream);
+    }
     H3_CHECK(fp4::quantize(&xc, &xs, x, format, x_tensor_scale, (cudaStream_t)stream));
     p.dependent = 1;
     return format == fp4::MX ? fp4::multiply<fp4::MX>(&xc, w_codes, p, (cudaStream_t)stream)

@@ -25,6 +25,7 @@ __all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_
 
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _FORMAT = {"mxfp4": 0, "nvfp4": 1}
+FUSED_ROWS = 8       # up to so many rows the product quantises x itself, without a workspace
 
 
 def _check_format(fmt: str) -> int:
@@ -249,8 +250,10 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
         raise ValueError(f"x has {cols} columns, the weight {weight.cols}")
     require_cuda(out, x, weight._buffer, bias)
     scale = _check_tensor_scale(weight.format, x_tensor_scale)
-    pitch, groups, chunks = _layout(rows, cols, weight.format)
-    work = x.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)   # x in 4 bits
+    work = None
+    if rows > FUSED_ROWS:
+        pitch, groups, chunks = _layout(rows, cols, weight.format)
+        work = x.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)   # x in 4 bits
     call("h3_linear_fp4", packed(o2), packed(x2), packed(work), weight.d_codes, weight.d_scales, packed(bias),
          _FORMAT[weight.format], scale, weight.tensor_scale, stream_of(x))
     return out

@@ -89,7 +89,8 @@ def test_entry_points_refuse_bad_arguments(h3):
 
     def linear(y, x, w, bias, fmt=1, tx=1.0, work=torch.zeros(4 * 32 + 512, dtype=torch.uint8)):
         b = None if bias is None else ctypes.byref(d(bias))
-        return lib.h3_linear_fp4(*[ctypes.byref(d(a)) for a in (y, x, work, w.codes, w.scales)], b, fmt, tx, 1.0, null)
+        args = [None if a is None else ctypes.byref(d(a)) for a in (y, x, work, w.codes, w.scales)]
+        return lib.h3_linear_fp4(*args, b, fmt, tx, 1.0, null)
 
     assert linear(y.float(), x, q, None) == 3
     assert linear(torch.zeros(4, 5, dtype=torch.bfloat16), x, q, None) == 2
@@ -100,6 +101,9 @@ def test_entry_points_refuse_bad_arguments(h3):
     assert linear(y, x, q, bias, tx=0.3) == 5
     assert linear(y, x, q, bias, work=torch.zeros(4 * 32 + 511, dtype=torch.uint8)) == 2    # a byte short
     assert linear(y, x, q, bias, work=torch.zeros(1000, dtype=torch.bfloat16)) == 3
+    assert linear(torch.zeros(9, 4, dtype=torch.bfloat16), torch.zeros(9, 48, dtype=torch.bfloat16), q, bias,
+                  work=None) == 1                                        # only up to 8 rows go without
+    assert linear(y.t(), x, q, bias, work=None) == 4
     empty = h3.fp4_empty(0, 48, "nvfp4", device="cpu")
     assert linear(torch.zeros(4, 0, dtype=torch.bfloat16), x, empty, None) == 0   # nothing to do
 
