@@ -376,7 +376,10 @@ int swap_split(int64_t tiles, int ktiles) {
         }
     }
     int split = ktiles < 8 ? ktiles : 8;
-    while (split > 1 && resident[dev][split].load() < tiles) --split;
+    // The count takes one CTA per SM, as if each used all of tensor memory; two run (their
+    // columns and shared memory fit).  Measured at 1 x 15360 x 5120 nvfp4: 14.6 us with a
+    // split for one per SM, 12.4 for two.
+    while (split > 1 && 2 * resident[dev][split].load() < tiles) --split;
     return split;
 }
 
@@ -685,10 +688,38 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     }
 }
 
+// CTA pairs resident at once.  0: cannot be told.
+template <int FMT>
+int resident_pairs() {
+    using C = Pair<FMT>;
+    static std::atomic<int> pairs[64];               // per device, once known
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return 0;
+    if (pairs[dev].load() == 0) {
+        auto kernel = tile_kernel<FMT>;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return 0;
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(2 * (num_sms() / 2));
+        cfg.blockDim = dim3(TILE_THREADS);
+        cfg.dynamicSmemBytes = C::SMEM;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return 0;
+        pairs[dev].store(n);
+    }
+    return pairs[dev].load();
+}
+
 template <int FMT>
 int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
     using C = Pair<FMT>;
-    auto kernel = tile_kernel<FMT>;
     CUtensorMap tx, tw, tsx, tsw;
     H3_CHECK(make_tmap_bytes(&tx, xc->data, xc->shape[1], xc->shape[0],
                              xc->shape[0] > 1 ? xc->strides[0] : xc->shape[1], 128, 128));
@@ -720,22 +751,11 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    static std::atomic<int> pairs[64];               // resident pairs per device, once known
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return H3_ERR_UNSUPPORTED;
-    if (pairs[dev].load() == 0) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-            return H3_ERR_LAUNCH;
-        cfg.gridDim = dim3(2 * (num_sms() / 2));
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return H3_ERR_LAUNCH;
-        pairs[dev].store(n);
-    }
-    const int tiles = p.num_m * p.num_n, slots = pairs[dev].load();
+    const int tiles = p.num_m * p.num_n, slots = resident_pairs<FMT>();
+    if (slots < 1) return H3_ERR_LAUNCH;
     cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
     cfg.numAttrs = p.dependent ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, tx, tw, tsx, tsw, ty, p) != cudaSuccess) {
+    if (cudaLaunchKernelEx(&cfg, tile_kernel<FMT>, tx, tw, tsx, tsw, ty, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;
     }
@@ -745,10 +765,29 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
 // 0 chooses per launch, 1 forces the swap form, 2 the tile form (h3_fp4_variant)
 std::atomic<int> g_variant{0};
 
+// Whether the swap form takes less time than the tile form, from times measured on B200
+// (us): a wave of tiles 0.47 per K tile and 1 to hand over, of the swap form's 128 x 128
+// tiles 0.62 per K tile of a CTA's share (0.82 in several waves); the rest of a launch 5.5
+// and 8.  Checked at M 17
+// to 2048, N 1000 to 27648, K 1000 to 13824: e.g. 256 x 5120 x 13824 swap 19.9, tiles 30;
+// 512 x 5120 x 5120 swap 20.1, tiles 15.9; 777 x 5120 x 5120 swap 21.4, tiles 26.7.
+template <int FMT>
+bool swap_form(const Params &p) {
+    if (p.M <= 128) return true;
+    const int64_t tiles = (int64_t)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+    const int64_t small = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128);
+    const int pairs = resident_pairs<FMT>(), split = swap_split<FMT, 128>(small, p.ktiles), slots = 2 * num_sms();
+    if (pairs < 1 || split < 1) return false;
+    const double in_tiles = 5.5 + (double)((tiles + pairs - 1) / pairs) * (p.ktiles * 0.47 + 1.0);
+    const double waves = (double)((small + slots - 1) / slots);
+    const double in_swap = 8.0 + waves * ((p.ktiles + split - 1) / split) * (waves > 1 ? 0.82 : 0.62);
+    return in_swap < in_tiles;
+}
+
 template <int FMT>
 int multiply(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_t stream) {
     const int v = g_variant.load();
-    if (v == 2 || (v == 0 && p.M > 128)) return launch_tiles<FMT>(xc, wc, p, stream);
+    if (v == 2 || (v == 0 && !swap_form<FMT>(p))) return launch_tiles<FMT>(xc, wc, p, stream);
     if (p.M <= 16) return launch_swap<FMT, 16, false>(xc, wc, p, stream);
     if (p.M <= 32) return launch_swap<FMT, 32, false>(xc, wc, p, stream);
     if (p.M <= 64) return launch_swap<FMT, 64, false>(xc, wc, p, stream);
