@@ -66,6 +66,16 @@ inline bool tensor_scale_ok(int fmt, float t) {
 // ---------------------------------------------------------------------------
 constexpr int UNIT = 16;
 
+struct TensorScale {
+    float t, sixth;              // a power of two, and 1 / (6 t)
+    __host__ static TensorScale make(float t) { return {t, 1.0f / (6.0f * t)}; }
+};
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // 16 columns of a row as packed BF16 pairs, zeros past the end
 template <bool VEC>
 __device__ __forceinline__ void load_unit(const __nv_bfloat16 *row, int col, int cols, uint32_t (&w)[8]) {
@@ -94,9 +104,15 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
     return r;
 }
 
+// e4m3 of v >= 0, at most 448.  Through fp16: where v is the quotient of an 8-bit amax and
+// 6 t, known to a few units of fp32, its 11 bits put a quotient that lies half way between
+// two e4m3 numbers (5 significant bits) exactly there, and any other, at least 2^-8 of
+// itself away, on its side.
 __device__ __forceinline__ uint32_t e4m3(float v) {
     uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
+    asm("{\n\t.reg .b32 h;\n\tcvt.rn.f16x2.f32 h, %1, %2;\n\tcvt.rn.satfinite.e4m3x2.f16x2 %0, h;\n\t}"
+        : "=h"(r)
+        : "f"(0.f), "f"(fminf(v, 448.f)));
     return r & 0xffu;
 }
 __device__ __forceinline__ float from_e4m3(uint32_t b) {
@@ -108,7 +124,7 @@ __device__ __forceinline__ float from_e4m3(uint32_t b) {
 // Codes (8 bytes) and scale byte of a unit; an mxfp4 block is this lane's unit and its
 // neighbour's (lane ^ 1), so all lanes of the warp take part.
 template <int FMT>
-__device__ __forceinline__ void quantize_unit(const uint32_t (&w)[8], float tensor_scale, uint32_t (&c)[2],
+__device__ __forceinline__ void quantize_unit(const uint32_t (&w)[8], const TensorScale &ts, uint32_t (&c)[2],
                                               uint32_t &byte) {
     // magnitudes order as integers; at 0x7f80 and above they are infinite or NaN
     uint32_t top2 = 0;
@@ -129,13 +145,13 @@ __device__ __forceinline__ void quantize_unit(const uint32_t (&w)[8], float tens
         }
     } else {
         const float amax = __uint_as_float(top << 16);
-        byte = bad ? 127u : e4m3(__fdiv_rn(amax, 6.0f * tensor_scale));
+        byte = bad ? 127u : e4m3(amax * ts.sixth);
         if (!bad && byte != 0) {
             // x / scale lies on a border between two codes, a multiple of 1/4, or (x has 8
             // significant bits, the scale 4) at least 1/300 of it away.  Adding and taking
-            // away 1.5 * 2^11 rounds the product with the reciprocal to a multiple of 2^-12,
-            // which puts the first kind exactly on its border and moves none across.
-            const float r = __frcp_rn(from_e4m3(byte) * tensor_scale);
+            // away 1.5 * 2^11 rounds the product with the (approximate) reciprocal to a multiple
+            // of 2^-12, which puts the first kind exactly on its border and moves none across.
+            const float r = rcp(from_e4m3(byte) * ts.t);
             constexpr float SNAP = 1.5f * 2048.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)

@@ -58,7 +58,7 @@ struct Params {
     const __nv_bfloat16 *x;
     int64_t ldx;
     int cols, x_vec;             // x_vec: 16-byte loads of x allowed
-    float x_scale;               // its tensor scale
+    TensorScale x_scale;
 };
 
 template <int FMT, int BN>
@@ -894,7 +894,7 @@ extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_te
         p.ldx = rows > 1 ? x->strides[0] : 0;
         p.cols = (int)cols;
         p.x_vec = aligned16(x->data) && p.ldx % 8 == 0;
-        p.x_scale = x_tensor_scale;
+        p.x_scale = fp4::TensorScale::make(x_tensor_scale);
         return format == fp4::MX ? fp4::multiply_fused<fp4::MX>(w_codes, p, (cudaStream_t)stream)
                                  : fp4::multiply_fused<fp4::NV>(w_codes, p, (cudaStream_t)stream);
     }
