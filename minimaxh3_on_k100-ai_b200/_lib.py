@@ -6,6 +6,7 @@ fallback implementation of any op.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 from pathlib import Path
@@ -13,6 +14,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libh3b200.so"
+HOST_PATH = LIB_PATH.with_name("_h3host.so")
 
 H3_OK = 0
 _STATUS = {
@@ -180,6 +182,29 @@ def call(name: str, *args) -> None:
     status = getattr(_lib or load(), name)(*args)   # ctypes passes an H3Tensor by reference
     if status:
         check(status, name)
+
+
+_HOST_ENTRIES = ("h3_quantize_fp4", "h3_dequantize_fp4", "h3_linear_fp4", "h3_cross_attention")
+_host = None
+
+
+def host():
+    """The extension that makes the regular calls of the small-launch operators without
+    ctypes (csrc/host_calls.cpp), bound to this library's entry points.  Its functions
+    return None for whatever is not in order; the caller then goes through ``call``, whose
+    checks raise.  False where it was not built: every call then goes through ``call``."""
+    global _host
+    if _host is None:
+        if HOST_PATH.exists():
+            spec = importlib.util.spec_from_file_location("_h3host", HOST_PATH)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            lib = load()
+            module.bind(*[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
+            _host = module
+        else:
+            _host = False
+    return _host
 
 
 def check_device(where: str) -> None:

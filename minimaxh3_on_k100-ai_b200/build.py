@@ -20,6 +20,7 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG.parent / "_build"
 LIB = PKG / "libh3b200.so"
+HOST = PKG / "_h3host.so"      # csrc/host_calls.cpp: the small operators' calls without ctypes
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -70,5 +71,32 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     return LIB
 
 
+def build_host(verbose: bool = False) -> Path:
+    """The Python extension over torch's C++ headers (the host compiler, no nvcc)."""
+    import sysconfig
+
+    import torch
+    src = CSRC / "host_calls.cpp"
+    newest = max(src.stat().st_mtime, (INCLUDE / "h3_b200.h").stat().st_mtime)
+    if HOST.exists() and HOST.stat().st_mtime >= newest:
+        return HOST
+    root = Path(torch.__path__[0])
+    cuda = Path(_nvcc()).resolve().parent.parent / "include"
+    includes = [sysconfig.get_path("include"), root / "include", root / "include/torch/csrc/api/include", cuda]
+    tmp = HOST.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{i}" for i in includes], str(src), "-o", str(tmp), f"-L{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building {HOST.name} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, HOST)
+    if verbose:
+        print(HOST)
+    return HOST
+
+
 if __name__ == "__main__":
     print(build(verbose="-v" in sys.argv))
+    print(build_host())

@@ -18,7 +18,7 @@ import math
 
 import torch
 
-from ._lib import call, packed, packed_bytes, require_cuda, stream_of
+from ._lib import CALLS, call, host, packed, packed_bytes, require_cuda, stream_of
 
 __all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_fp4", "quantize_fp4_", "dequantize_fp4",
            "dequantize_fp4_", "pack_fp4", "unpack_fp4", "linear_fp4", "linear_fp4_"]
@@ -67,13 +67,19 @@ class Fp4Tensor:
     @classmethod
     def _uninitialised(cls, like: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
         """On ``like``'s device, codes and scales in one allocation."""
-        self = cls.__new__(cls)
-        self.rows, self.cols, self.format, self.tensor_scale = rows, cols, format, tensor_scale
         pitch, groups, chunks = _layout(rows, cols, format)
-        self._buffer = buf = like.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)
+        buf = like.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)
         at = buf.data_ptr()
-        self.d_codes = packed_bytes(at, (rows, pitch), (pitch, 1))
-        self.d_scales = packed_bytes(at + rows * pitch, (groups, chunks, 512), (chunks * 512, 512, 1))
+        return cls._of(buf, packed_bytes(at, (rows, pitch), (pitch, 1)),
+                       packed_bytes(at + rows * pitch, (groups, chunks, 512), (chunks * 512, 512, 1)), rows, cols,
+                       format, tensor_scale)
+
+    @classmethod
+    def _of(cls, buffer, d_codes, d_scales, rows, cols, format, tensor_scale) -> Fp4Tensor:
+        """Of a buffer laid out as ``_uninitialised`` does."""
+        self = cls.__new__(cls)
+        self._buffer, self.d_codes, self.d_scales, self.rows, self.cols = buffer, d_codes, d_scales, rows, cols
+        self.format, self.tensor_scale = format, tensor_scale
         self._codes = self._scales = None
         return self
 
@@ -159,6 +165,10 @@ def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: float = 1
     """x [..., cols] BF16 as a 4-bit matrix of its rows."""
     code = _check_format(format)
     scale = _check_tensor_scale(format, tensor_scale)
+    fast = host() and host().quantize_fp4(x, code, scale)
+    if fast:
+        CALLS["n"] += 1
+        return Fp4Tensor._of(*fast, format, scale)
     require_cuda(x)
     x2 = _rows_of(x)
     rows, cols = x2.shape
@@ -180,6 +190,12 @@ def dequantize_fp4_(out: torch.Tensor, q: Fp4Tensor) -> torch.Tensor:
 
 def dequantize_fp4(q: Fp4Tensor) -> torch.Tensor:
     """The values a 4-bit matrix stands for, [rows, cols] BF16 (exact)."""
+    if host():
+        out = host().dequantize_fp4(q._buffer, q.d_codes, q.d_scales, q.rows, q.cols, _FORMAT[q.format],
+                                    q.tensor_scale)
+        if out is not None:
+            CALLS["n"] += 1
+            return out
     return dequantize_fp4_(q._buffer.new_empty((q.rows, q.cols), dtype=torch.bfloat16), q)
 
 
@@ -261,6 +277,14 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
 
 def linear_fp4(x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
                x_tensor_scale: float = 1.0) -> torch.Tensor:
+    """``linear_fp4_`` into a new tensor."""
+    if host() and not isinstance(x, Fp4Tensor):
+        out = host().linear_fp4(x, weight._buffer, weight.d_codes, weight.d_scales, weight.rows, weight.cols, bias,
+                                _FORMAT[weight.format], _check_tensor_scale(weight.format, x_tensor_scale),
+                                weight.tensor_scale, FUSED_ROWS)
+        if out is not None:
+            CALLS["n"] += 1
+            return out
     lead = (x.rows,) if isinstance(x, Fp4Tensor) else x.shape[:-1]
     out = weight._buffer.new_empty((*lead, weight.rows), dtype=torch.bfloat16)
     return linear_fp4_(out, x, weight, bias, x_tensor_scale)

@@ -20,7 +20,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import call, desc, packed, require_cuda, stream_of
+from ._lib import CALLS, call, desc, host, packed, require_cuda, stream_of
 
 __all__ = [
     "h3_rms_norm", "h3_rms_norm_", "h3_swiglu", "h3_swiglu_", "h3_rms_modulate", "h3_rms_modulate_",
@@ -204,6 +204,12 @@ def cross_attention_(out, q, k, v, lengths=None, scale=None):
 
 
 def cross_attention(q, k, v, lengths=None, scale=None):
+    """``cross_attention_`` into a new tensor."""
+    if host():
+        out = host().cross_attention(q, k, v, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
+        if out is not None:
+            CALLS["n"] += 1
+            return out
     return cross_attention_(q.new_empty(q.shape), q, k, v, lengths, scale)
 
 

@@ -21,7 +21,13 @@ DEV = "cuda"
 def h3():
     import h3b200
     h3b200.load()
+    assert h3b200._lib.host(), "the host extension is not built"
     return h3b200
+
+
+@pytest.fixture
+def ctypes_only(h3, monkeypatch):
+    monkeypatch.setattr(h3._lib, "_host", False)
 
 
 @pytest.fixture(params=[1, 2], ids=["rows", "tiles"])
@@ -252,3 +258,20 @@ def test_graph_and_streams(h3, form):
     torch.cuda.synchronize()
     for got, ref in zip(outs, want):
         assert all(torch.equal(o, ref) for o in got)
+
+
+def test_both_ways_of_calling_agree(h3, monkeypatch):
+    q, k, v = _inputs(3, 20, 90, 4, 2, seed=14)
+    lengths = torch.tensor([90, 0, 17], device=DEV)
+    calls = (lambda: h3.cross_attention(q, k, v), lambda: h3.cross_attention(q, k, v, lengths),
+             lambda: h3.cross_attention(q[:, ::2], k, v, lengths, scale=0.2),
+             lambda: h3.cross_attention(q.transpose(1, 2)[:, :2].transpose(1, 2), k, v),
+             lambda: h3.cross_attention(q, k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)))
+    fast = [f() for f in calls]
+    monkeypatch.setattr(h3._lib, "_host", False)
+    for f, a in zip(calls, fast):
+        assert torch.equal(f(), a)
+
+
+def test_refusals_without_the_extension(h3, ctypes_only):
+    test_refusals(h3)

@@ -24,7 +24,13 @@ FORMATS = ("mxfp4", "nvfp4")
 def h3():
     import h3b200
     h3b200.load()
+    assert h3b200._lib.host(), "the host extension is not built"
     return h3b200
+
+
+@pytest.fixture
+def ctypes_only(h3, monkeypatch):
+    monkeypatch.setattr(h3._lib, "_host", False)
 
 
 def _parts(h3, q):
@@ -295,3 +301,42 @@ def test_graph_and_streams(h3, form):
     for got, ref in zip(outs, want):
         assert all(torch.equal(y, ref) for y in got)
     assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_both_ways_of_calling_agree(h3, monkeypatch, fmt):
+    """The extension's calls and the ctypes ones: the same bits, shapes and errors."""
+    x = torch.randn(3, 41, 700, device=DEV).bfloat16()
+    w = _weight(h3, 100, 700, fmt, 7)
+    bias = torch.randn(100, device=DEV).bfloat16()
+    inputs = (x, x[0], x[0, :5], x[:, :, 5:], x[0, :, 5:], x[0, 1:2], x[:0], x.transpose(0, 1))
+
+    def all_of(t):
+        q = h3.quantize_fp4(t, fmt)
+        p = h3.quantize_fp4(torch.nn.functional.pad(t, (0, 700 - t.shape[-1])), fmt)
+        y = h3.linear_fp4(torch.nn.functional.pad(t, (0, 700 - t.shape[-1])), w, bias)
+        return [*h3.unpack_fp4(q), h3.dequantize_fp4(q), h3.linear_fp4(p, w, bias), y, y.new_tensor(y.shape)]
+
+    n = h3._lib.CALLS["n"]
+    fast = [all_of(t) for t in inputs]
+    made = h3._lib.CALLS["n"] - n
+    monkeypatch.setattr(h3._lib, "_host", False)
+    n = h3._lib.CALLS["n"]
+    slow = [all_of(t) for t in inputs]
+    assert h3._lib.CALLS["n"] - n == made
+    for a, b in zip(fast, slow):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_refusals_without_the_extension(h3, ctypes_only):
+    test_linear_refusals(h3)
+
+
+def test_other_device_is_refused(h3):
+    """Tensors of a device that is not the current one (here: the CPU) never reach a launch."""
+    w = _weight(h3, 64, 64, "nvfp4", 4)
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for f in (lambda: h3.linear_fp4(x, w), lambda: h3.quantize_fp4(x),
+              lambda: h3.linear_fp4(x.to(DEV), w, bias=torch.zeros(64, dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            f()
