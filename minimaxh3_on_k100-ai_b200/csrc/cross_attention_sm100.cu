@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         tmem_alloc(tmem_slot, C::TMEM);
         tmem_relinquish();
     }
+    wait_for_previous();
     if (p.ordered) {
         // samples by their number of key tiles, most first (their rank by counting)
         int *cost = reinterpret_cast<int *>(smem + C::OFF_Q);
@@ -561,6 +562,15 @@ __global__ void __launch_bounds__(Rows<MT, WARPS>::THREADS)
     y /= p.chunks;
     const int kh = y % p.kv_heads, b = y / p.kv_heads;            // b = 0 where the batch is folded
     const int row0 = chunk * C::ROWS, rows = min(C::ROWS, p.rows - row0);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], ROW_WARPS);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    wait_for_previous();
     const int len = states(p, b);
     const int tiles = (len + KEYS - 1) / KEYS;
     const int t0 = (int)((int64_t)tiles * rank / split), t1 = (int)((int64_t)tiles * (rank + 1) / split);
@@ -576,14 +586,6 @@ __global__ void __launch_bounds__(Rows<MT, WARPS>::THREADS)
         return bb * sb + s * ss + (int64_t)(kh * p.group + (g - s * p.group)) * sh;
     };
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], ROW_WARPS);
-        }
-        *abort_flag = 0;
-        fence_mbar_init();
-    }
     __syncthreads();
 
     if (warp == ROW_WARPS) {
@@ -878,7 +880,18 @@ int launch_tiles(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, c
     const int grid = p.items < num_sms() ? p.items : num_sms();
     // with a length per sample items differ in cost: dealt in descending order they level out
     p.ordered = p.lens && p.B > 1 && p.B <= cross::MAX_ORDERED && p.items > grid;
-    cross::tile_kernel<NQ><<<grid, cross::TILE_THREADS, C::SMEM, stream>>>(tq, tk, tv, to, p);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = overlapped_launch();
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(cross::TILE_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, cross::tile_kernel<NQ>, tq, tk, tv, to, p) != cudaSuccess) {
+        cudaGetLastError();
+        return H3_ERR_LAUNCH;
+    }
     return launch_status();
 }
 
@@ -946,9 +959,11 @@ int launch_rows(const h3_tensor *k, const h3_tensor *v, cross::Params &p, cudaSt
     const int split = rows_split<MT, WARPS>(groups, p.Sk);
     if (split < 1) return H3_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    rows_config<MT, WARPS>(&cfg, &attr);
-    attr.val.clusterDim.x = split;
+    cudaLaunchAttribute attr[2];
+    rows_config<MT, WARPS>(&cfg, attr);
+    attr[0].val.clusterDim.x = split;
+    attr[1] = overlapped_launch();
+    cfg.numAttrs = 2;
     cfg.gridDim = dim3(split, (unsigned)groups, 1);
     cfg.stream = stream;
     if (cudaLaunchKernelEx(&cfg, cross::rows_kernel<MT, WARPS>, tk, tv, p) != cudaSuccess) {

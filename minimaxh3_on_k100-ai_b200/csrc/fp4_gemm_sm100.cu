@@ -53,7 +53,7 @@ struct Params {
     float t;
     int num_m, num_n;            // tiles
     int wide;                    // 4-column (8-byte) stores allowed
-    int dependent;               // launched behind the quantisation of x: only w may be read before it ends
+    int dependent;               // launched behind the quantisation of x: w may be read before that ends
     // fused quantisation: x itself
     const __nv_bfloat16 *x;
     int64_t ldx;
@@ -138,7 +138,9 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
         }
         __syncwarp();
     };
-    // the weights wait for nothing: warp 0 fills the ring with them before the rest is set up
+    // Warp 0 fills the ring with weights before the rest is set up: behind the quantisation
+    // of x at once (whatever ran before that kernel is done), else when the kernel before
+    // this one has ended.
     const int head = min(nk, C::STAGES);
     if (warp == 0) {
         if (elect_one()) {
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             fence_proxy_async_smem();   // the copies below come before any block barrier
         }
         __syncwarp();
+        if (!p.dependent) wait_for_previous();
         for (int i = 0; i < head; ++i) load_w(i);
     } else if (warp == 1) {
         tmem_alloc(tmem_slot, C::TMEM);
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             }
             __syncwarp();
         };
-        if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (p.dependent) wait_for_previous();
         for (int i = 0; i < head; ++i) load_x(i);
         for (int i = head; i < nk; ++i) {
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, abort_flag))) break;
@@ -246,6 +249,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             }
         };
         const int first = warp - 4;
+        wait_for_previous();
         if (first < nk) load(first);
         for (int i = first; i < nk; i += QUANT_WARPS) {
             const int slot = i % C::STAGES;
@@ -404,14 +408,13 @@ int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_
     attr[0].val.clusterDim.x = split;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[1] = overlapped_launch();
     cfg.gridDim = dim3(split, p.num_n, p.num_m);
     cfg.blockDim = dim3(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0));
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = p.dependent ? 2 : 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, swap_kernel<FMT, BN, FUSED>, tx, tw, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;
@@ -503,7 +506,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             tma_prefetch_desc(&tsx);
             tma_prefetch_desc(&tsw);
         }
-        if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        wait_for_previous();
         uint32_t it = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles && ok; tile += step) {
@@ -590,6 +593,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const int wq = warp & 3;
         uint8_t *buf0 = smem + C::OFF_STORE + wq * 2 * C::STORE;
         const uint32_t bias = smem_u32(smem + C::OFF_BIAS + wq * 512);
+        wait_for_previous();             // the bias, and y, may be the previous kernel's
         uint32_t lt = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles; tile += step, ++lt) {
@@ -744,17 +748,15 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[1] = overlapped_launch();
     cfg.blockDim = dim3(TILE_THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
     const int tiles = p.num_m * p.num_n, slots = resident_pairs<FMT>();
     if (slots < 1) return H3_ERR_LAUNCH;
     cfg.gridDim = dim3(2 * (tiles < slots ? tiles : slots));
-    cfg.numAttrs = p.dependent ? 2 : 1;
+    cfg.numAttrs = 2;
     if (cudaLaunchKernelEx(&cfg, tile_kernel<FMT>, tx, tw, tsx, tsw, ty, p) != cudaSuccess) {
         cudaGetLastError();
         return H3_ERR_LAUNCH;

@@ -101,7 +101,10 @@ __device__ __forceinline__ void store_segment(__nv_bfloat16 *dst, const uint16_t
 template <int FMT, bool VEC>
 __global__ void __launch_bounds__(THREADS)
     quantize_kernel(const __nv_bfloat16 *x, uint8_t *codes, uint8_t *scales, Shape s) {
-    asm volatile("griddepcontrol.launch_dependents;");   // a product waiting on this may set itself up
+    // in this order: a product behind this kernel reads its weights ahead of the wait for x,
+    // so nothing before this kernel may still be running when that product starts
+    wait_for_previous();
+    release_next();
     const int tx = 1 << s.log_tx;
     const int unit = (int)blockIdx.y * tx + (int)(threadIdx.x & (tx - 1));
     const int64_t row = (int64_t)blockIdx.x * (THREADS >> s.log_tx) + (threadIdx.x >> s.log_tx);
@@ -168,6 +171,7 @@ __global__ void __launch_bounds__(THREADS)
     const int unit = (int)blockIdx.y * tx + (int)(threadIdx.x & (tx - 1));
     const int64_t row = (int64_t)blockIdx.x * (THREADS >> s.log_tx) + (threadIdx.x >> s.log_tx);
     const int col = unit * UNIT;
+    wait_for_previous();
     const bool live = row < s.rows && col < s.cols;
     if (VEC && !live) return;
     uint32_t w[8];
@@ -222,6 +226,22 @@ int plan(const h3_tensor *x, const h3_tensor *codes, const h3_tensor *scales, in
     return H3_OK;
 }
 
+template <typename Kernel, typename... Args>
+int launch(Kernel kernel, dim3 grid, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = overlapped_launch();
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) {
+        cudaGetLastError();
+        return H3_ERR_LAUNCH;
+    }
+    return launch_status();
+}
+
 int quantize(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int fmt, float tensor_scale,
              cudaStream_t stream) {
     Shape s{};
@@ -231,9 +251,8 @@ int quantize(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x
     if (x->shape[0] == 0) return H3_OK;
     auto kernel = fmt == MX ? (vec ? quantize_kernel<MX, true> : quantize_kernel<MX, false>)
                             : (vec ? quantize_kernel<NV, true> : quantize_kernel<NV, false>);
-    kernel<<<grid, THREADS, 0, stream>>>(static_cast<const __nv_bfloat16 *>(x->data),
-                                         static_cast<uint8_t *>(codes->data), static_cast<uint8_t *>(scales->data), s);
-    return launch_status();
+    return launch(kernel, grid, stream, static_cast<const __nv_bfloat16 *>(x->data),
+                  static_cast<uint8_t *>(codes->data), static_cast<uint8_t *>(scales->data), s);
 }
 
 }  // namespace fp4
@@ -256,8 +275,6 @@ extern "C" int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, con
     if (y->shape[0] > 1 && y->strides[0] < y->shape[1]) return H3_ERR_BAD_LAYOUT;   // rows would overlap
     auto kernel = format == fp4::MX ? (vec ? fp4::dequantize_kernel<fp4::MX, true> : fp4::dequantize_kernel<fp4::MX, false>)
                                     : (vec ? fp4::dequantize_kernel<fp4::NV, true> : fp4::dequantize_kernel<fp4::NV, false>);
-    kernel<<<grid, fp4::THREADS, 0, (cudaStream_t)stream>>>(static_cast<__nv_bfloat16 *>(y->data),
-                                                            static_cast<const uint8_t *>(codes->data),
-                                                            static_cast<const uint8_t *>(scales->data), s);
-    return launch_status();
+    return fp4::launch(kernel, grid, (cudaStream_t)stream, static_cast<__nv_bfloat16 *>(y->data),
+                       static_cast<const uint8_t *>(codes->data), static_cast<const uint8_t *>(scales->data), s);
 }

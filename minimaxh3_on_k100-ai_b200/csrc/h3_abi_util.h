@@ -84,6 +84,14 @@ inline int launch_status() {
     return e == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
 }
 
+// Launch attribute of kernels that call wait_for_previous() (sm100_ptx.cuh).
+inline cudaLaunchAttribute overlapped_launch() {
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
 // SM count of the current device, cached per device ordinal.
 inline int num_sms() {
     static std::atomic<int> cache[64];

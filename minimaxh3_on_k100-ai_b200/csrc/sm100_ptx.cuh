@@ -131,6 +131,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched with overlapped_launch() is set up while
+// the one before it in its stream drains, and calls wait_for_previous() before it touches
+// memory that may be that kernel's (all of it is visible afterwards); release_next() lets
+// the kernel after it start its set-up already.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // After an abort: give copies and MMAs already in flight time to land before
 // the CTA releases its TMEM and shared memory (bounded, ~1 ms).
 __device__ __forceinline__ void drain_in_flight() {

@@ -275,3 +275,23 @@ def test_both_ways_of_calling_agree(h3, monkeypatch):
 
 def test_refusals_without_the_extension(h3, ctypes_only):
     test_refusals(h3)
+
+
+def test_calls_back_to_back(h3, form):
+    """Each call overlaps the end of the kernel before it, which writes its inputs."""
+    for Sq in (1, 20, 300):
+        sets = [_inputs(3, Sq, 200, 4, 2, seed=20 + i) for i in range(4)]
+        lens = [torch.tensor(n, device=DEV) for n in ([200, 3, 0], [1, 200, 64], [0, 0, 129], [77, 128, 200])]
+        want = []
+        for (q, k, v), n in zip(sets, lens):
+            torch.cuda.synchronize()
+            want.append(h3.cross_attention(q, k, v, n))
+        torch.cuda.synchronize()
+        q, n, out = torch.zeros_like(sets[0][0]), torch.zeros_like(lens[0]), torch.zeros_like(want[0])
+        k, v = torch.zeros_like(sets[0][1]), torch.zeros_like(sets[0][2])
+        got = []
+        for i in range(40):
+            for dst, src in ((k, sets[i % 4][1]), (v, sets[i % 4][2]), (n, lens[i % 4]), (q, sets[i % 4][0])):
+                dst.copy_(src)
+            got.append(h3.cross_attention_(out, q, k, v, n).clone())
+        assert all(torch.equal(o, want[i % 4]) for i, o in enumerate(got))

@@ -340,3 +340,37 @@ def test_other_device_is_refused(h3):
               lambda: h3.linear_fp4(x.to(DEV), w, bias=torch.zeros(64, dtype=torch.bfloat16))):
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize("M", [1, 4, 12, 40, 300, 1500])
+def test_calls_back_to_back(h3, M):
+    """Kernels overlap the end of the one before them in the stream; what that one writes --
+    the weights, the rows, the bias, all into the same buffers every time -- must be seen,
+    and what it still reads must not be overwritten."""
+    for fmt in FORMATS:
+        ws = [(torch.randn(640, 1100, device=DEV) * 0.02).bfloat16() for _ in range(6)]
+        xs = [torch.randn(M, 1100, device=DEV).bfloat16() for _ in range(6)]
+        bs = [torch.randn(640, device=DEV).bfloat16() for _ in range(6)]
+        want = []
+        for w, x, b in zip(ws, xs, bs):
+            torch.cuda.synchronize()
+            q = h3.quantize_fp4(w, fmt)
+            torch.cuda.synchronize()
+            want.append(h3.linear_fp4(x, q, b))
+            torch.cuda.synchronize()
+        weight, x, bias = h3.fp4_empty(640, 1100, fmt), torch.zeros_like(xs[0]), torch.zeros_like(bs[0])
+        xq, y = h3.fp4_empty(M, 1100, fmt), torch.zeros_like(want[0])
+        got = []
+        for i in range(60):
+            bias.copy_(bs[i % 6])
+            x.copy_(xs[i % 6])
+            h3.quantize_fp4_(weight, ws[i % 6])
+            h3.linear_fp4_(y, x, weight, bias)
+            got.append(y.clone())
+            if M > 8:
+                h3.quantize_fp4_(xq, x)
+                h3.linear_fp4_(y, xq, weight, bias)
+                got.append(y.clone())
+        per = 2 if M > 8 else 1
+        assert all(torch.equal(o, want[i // per % 6]) for i, o in enumerate(got))
+    assert h3.load().h3_device_error() == 0
