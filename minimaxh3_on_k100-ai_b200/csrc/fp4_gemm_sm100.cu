@@ -101,6 +101,11 @@ __device__ __forceinline__ void ld_shared_words(uint32_t addr, uint32_t (&r)[4])
                  : "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ uint32_t ld_shared_word(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void st_shared_words(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -426,7 +431,8 @@ int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_
 // tile form: persistent CTA pairs, 256 x 256 output tiles
 // ---------------------------------------------------------------------------
 constexpr int TILE = 256;                        // rows and columns of a pair's output tile
-constexpr int TILE_THREADS = 256;
+constexpr int EPI_WARPS = 8;                     // two per quarter of the rows, each every other 64 columns
+constexpr int TILE_THREADS = (4 + EPI_WARPS) * 32;
 constexpr int GROUP_N = 8;                       // column tiles per raster group
 
 template <int FMT>
@@ -438,10 +444,10 @@ struct Pair {
     static constexpr int OFF_SFB = OFF_SFA + SF_BYTES;        // all 256 w rows: each CTA multiplies with every one
     static constexpr int STAGE = OFF_SFB + 2 * SF_BYTES;      // a multiple of 1024
     static constexpr int STAGES = 5;
-    static constexpr int STORE = 32 * 128;                    // 32 rows x 64 columns of y, two per epilogue warp
+    static constexpr int STORE = 32 * 128;                    // 32 rows x 64 columns of y, per epilogue warp
     static constexpr int OFF_STORE = STAGES * STAGE;
-    static constexpr int OFF_BIAS = OFF_STORE + 8 * STORE;    // the tile's bias, a copy per epilogue warp
-    static constexpr int OFF_BAR = OFF_BIAS + 4 * 512;
+    static constexpr int OFF_BIAS = OFF_STORE + EPI_WARPS * STORE;   // the bias of those columns
+    static constexpr int OFF_BAR = OFF_BIAS + EPI_WARPS * 128;
     static constexpr int SMEM = OFF_BAR + (2 * STAGES + 2) * 8 + 16 + 1024;
     static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
     // Tensor memory: two 256-column accumulators sharing 128 columns, and two buffers of
@@ -486,7 +492,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             mbar_init(&empty[s], 1);
         }
         mbar_init(acc_full, 1);
-        mbar_init(acc_free, 8);
+        mbar_init(acc_free, 2 * EPI_WARPS);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -590,9 +596,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
         if (!ok) drain_in_flight();
     } else if (warp >= 4) {
-        const int wq = warp & 3;
-        uint8_t *buf0 = smem + C::OFF_STORE + wq * 2 * C::STORE;
-        const uint32_t bias = smem_u32(smem + C::OFF_BIAS + wq * 512);
+        const int wq = warp & 3, half = (warp - 4) >> 2;
+        uint8_t *buf = smem + C::OFF_STORE + (warp - 4) * C::STORE;
+        const uint32_t bias = smem_u32(smem + C::OFF_BIAS + (warp - 4) * 128);
         wait_for_previous();             // the bias, and y, may be the previous kernel's
         uint32_t lt = 0;
         bool ok = true;
@@ -600,52 +606,50 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             int m, n;
             tile_at(p, tile, m, n);
             const int row0 = m * TILE + (int)rank * 128 + wq * 32;      // this warp's first row
-            if (p.bias) {
-                uint16_t b[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int col = n * TILE + lane * 8 + i;
-                    b[i] = col < p.N ? __ldg(reinterpret_cast<const uint16_t *>(p.bias) + col) : (uint16_t)0;
-                }
-                st_shared_words(bias + lane * 16, b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16,
-                                b[4] | (uint32_t)b[5] << 16, b[6] | (uint32_t)b[7] << 16);
-                __syncwarp();
-            }
             ok = __all_sync(0xffffffffu, mbar_wait(acc_full, lt & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
             const uint32_t acc = tmem + ((lt & 1) ? C::ACC1 : 0) + ((uint32_t)(wq * 32) << 16);
-            // 64 columns at a time, the shared ones first (the end of accumulator 0, the start
-            // of accumulator 1); once they are in registers the next tile may start
+            // 64 columns at a time, of the shared ones first (the end of accumulator 0, the start
+            // of accumulator 1); once those are in registers the next tile may start
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-                const int c0 = ((lt & 1) ? i : i ^ 2) * 64, col = n * TILE + c0;
+            for (int i = 0; i < 2; ++i) {
+                const int c0 = (((lt & 1) ? 2 * i : 2 - 2 * i) + half) * 64, col = n * TILE + c0;
                 uint32_t v[2][32];
                 tmem_ld32(acc + c0, v[0]);
                 tmem_ld32(acc + c0 + 32, v[1]);
+                uint16_t b0 = 0, b1 = 0;
+                if (p.bias) {
+                    const uint16_t *b = reinterpret_cast<const uint16_t *>(p.bias) + col + 2 * lane;
+                    if (col + 2 * lane < p.N) b0 = __ldg(b);
+                    if (col + 2 * lane + 1 < p.N) b1 = __ldg(b + 1);
+                }
                 tmem_ld_wait();
-                if (i == 1) {
+                if (i == 0) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(mapa_shared(acc_free, 0));
                 }
                 if (col >= p.N || row0 >= p.M) continue;                // uniform over the warp
+                if (p.bias) {
+                    st_shared_f32(bias + lane * 4, b0 | (uint32_t)b1 << 16);
+                    __syncwarp();
+                }
                 uint32_t w[32];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint32_t b[4] = {0, 0, 0, 0};
-                        if (p.bias) ld_shared_words(bias + (c0 + 32 * h + 8 * q) * 2, b);
+                        if (p.bias) ld_shared_words(bias + (32 * h + 8 * q) * 2, b);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             w[16 * h + 4 * q + e] = bf2u(
                                 __floats2bfloat162_rn(fmaf(__uint_as_float(v[h][8 * q + 2 * e]), p.t, blo(b[e])),
                                                       fmaf(__uint_as_float(v[h][8 * q + 2 * e + 1]), p.t, bhi(b[e]))));
                     }
-                uint8_t *buf = buf0 + (i & 1) * C::STORE;
                 if (p.wide) {
-                    if (lane == 0) tma_store_wait_read_1();              // the store two blocks back has read it
+                    if (lane == 0) tma_store_wait_read();                // the last store has read the buffer
                     __syncwarp();
                 }
                 // 16-byte piece q of row r at q ^ (r & 7): the layout the TMA store reads
@@ -661,18 +665,18 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                         tma_store_commit();
                     }
                 } else {
-                    // rows too odd for TMA: two columns per lane, a row at a time
+                    // Rows too odd for TMA: two columns per lane, a row at a time.  (4-byte words
+                    // across neighbouring lanes where the row starts half way into one took
+                    // longer: 13.9 us against 11.9 at 333 x 4861 x 1795.)
                     __syncwarp();
-                    const int rows = min(32, p.M - row0);
-                    for (int r = 0; r < rows; ++r) {
-                        uint32_t o;
-                        asm volatile("ld.shared.b32 %0, [%1];"
-                                     : "=r"(o)
-                                     : "r"(smem_u32(buf) + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)
-                                     : "memory");
-                        uint16_t *dst = reinterpret_cast<uint16_t *>(p.y) + (int64_t)(row0 + r) * p.ldy + col + 2 * lane;
-                        if (col + 2 * lane < p.N) dst[0] = (uint16_t)o;
-                        if (col + 2 * lane + 1 < p.N) dst[1] = (uint16_t)(o >> 16);
+                    const int rows = min(32, p.M - row0), left = p.N - col - 2 * lane;
+                    const uint32_t at = smem_u32(buf) + (lane & 3) * 4;
+                    uint16_t *dst = reinterpret_cast<uint16_t *>(p.y) + (int64_t)row0 * p.ldy + col + 2 * lane;
+#pragma unroll 4
+                    for (int r = 0; r < rows; ++r, dst += p.ldy) {
+                        const uint32_t o = ld_shared_word(at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4));
+                        if (left > 0) dst[0] = (uint16_t)o;
+                        if (left > 1) dst[1] = (uint16_t)(o >> 16);
                     }
                     __syncwarp();
                 }
