@@ -433,7 +433,9 @@ int launch_swap(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream_
 constexpr int TILE = 256;                        // rows and columns of a pair's output tile
 constexpr int EPI_WARPS = 8;                     // two per quarter of the rows, each every other 64 columns
 constexpr int TILE_THREADS = (4 + EPI_WARPS) * 32;
-constexpr int GROUP_N = 8;                       // column tiles per raster group
+// Column tiles per raster group.  Sustained at 18944 x 27648 x 5120 nvfp4, under the power cap:
+// groups of 4 / 8 / 20 / 32 / 64 / all ran 1385 / 1362 / 1336 / 1328 / 1350 / 1483 us.
+constexpr int GROUP_N = 32;
 
 template <int FMT>
 struct Pair {
