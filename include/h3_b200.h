@@ -192,7 +192,7 @@ int h3_mha_scatter(const h3_tensor *dsts, int32_t ndst, const h3_tensor *q, cons
  * number of states of each sample (clamped to [0, Sk]), or NULL for Sk.  Non-causal,
  * fp32 softmax and accumulation, P rounded to BF16.  States behind a sample's length are
  * not read into a result whatever they hold; a sample without states, and a row whose
- * scores are all -inf, gets zeros.  scale positive and finite.  Layout rules of h3_mha.
+ * scores are all -inf, gets zeros.  out may not overlap k or v.  scale positive and finite.  Layout rules of h3_mha.
  * No reference counterpart (its attention, h3_mha, has one key length and equal heads). */
 int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, const h3_tensor *v,
                        const h3_tensor *lengths, float scale, void *stream);
@@ -338,7 +338,7 @@ int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tenso
  * 16-byte aligned, any contents, at least as many bytes as x's codes and scales together)
  * and multiplied with the 4-bit weight [N,K] of the same format; fp32 accumulation, one
  * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1.
- * With a NULL workspace (at most 8 rows) the product quantises x itself, in one launch;
+ * y may not overlap an input.  With a NULL workspace (at most 8 rows, N at most 8388480) the product quantises x itself, in one launch;
  * the results are those of form 1 of h3_fp4_variant. */
 int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace, const h3_tensor *w_codes,
                   const h3_tensor *w_scales, const h3_tensor *bias, int32_t format, float x_tensor_scale,

@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();   // every warp: the bounded waits below must not count the previous kernel's time
 
     if (warp == 0) {
         auto load_x = [&](int i) {
@@ -182,7 +183,6 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             }
             __syncwarp();
         };
-        if (p.dependent) wait_for_previous();
         for (int i = 0; i < head; ++i) load_x(i);
         for (int i = head; i < nk; ++i) {
             if (!__all_sync(0xffffffffu, mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, abort_flag))) break;
@@ -254,7 +254,6 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             }
         };
         const int first = warp - 4;
-        wait_for_previous();
         if (first < nk) load(first);
         for (int i = first; i < nk; i += QUANT_WARPS) {
             const int slot = i % C::STAGES;
@@ -506,6 +505,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    wait_for_previous();   // every warp: the bounded waits below must not count the previous kernel's time
 
     if (warp == 0) {
         if (elect_one()) {
@@ -514,7 +514,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             tma_prefetch_desc(&tsx);
             tma_prefetch_desc(&tsw);
         }
-        wait_for_previous();
         uint32_t it = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles && ok; tile += step) {
@@ -601,7 +600,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const int wq = warp & 3, half = (warp - 4) >> 2;
         uint8_t *buf = smem + C::OFF_STORE + (warp - 4) * C::STORE;
         const uint32_t bias = smem_u32(smem + C::OFF_BIAS + (warp - 4) * 128);
-        wait_for_previous();             // the bias, and y, may be the previous kernel's
         uint32_t lt = 0;
         bool ok = true;
         for (int tile = first; tile < num_tiles; tile += step, ++lt) {
@@ -781,6 +779,7 @@ std::atomic<int> g_variant{0};
 // 512 x 5120 x 5120 swap 20.1, tiles 15.9; 777 x 5120 x 5120 swap 21.4, tiles 26.7.
 template <int FMT>
 bool swap_form(const Params &p) {
+    if ((p.N + 127) / 128 > 65535) return false;     // its grid's limit
     if (p.M <= 128) return true;
     const int64_t tiles = (int64_t)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
     const int64_t small = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128);

@@ -295,3 +295,17 @@ def test_calls_back_to_back(h3, form):
                 dst.copy_(src)
             got.append(h3.cross_attention_(out, q, k, v, n).clone())
         assert all(torch.equal(o, want[i % 4]) for i, o in enumerate(got))
+
+
+def test_offsets_past_32_bits(h3):
+    """More than 2^31 elements of keys and values; the last states and heads count."""
+    q = torch.randn(1, 1, 128, 128, device=DEV).bfloat16()
+    kv = torch.zeros(1, 70000, 2, 128, 128, dtype=torch.bfloat16, device=DEV)
+    kv[:, -50:] = torch.randn(1, 50, 2, 128, 128, device=DEV).bfloat16()
+    kv[:, :, 0, 126:] = torch.randn(1, 70000, 2, 128, device=DEV).bfloat16()
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    out = h3.cross_attention(q, k, v)
+    _check(h3, out[:, :, 126:], q[:, :, 126:], k[:, :, 126:], v[:, :, 126:])
+    q2 = torch.randn(1, 200, 128, 128, device=DEV).bfloat16()
+    out = h3.cross_attention(q2, k, v)
+    _check(h3, out[:, :, 126:], q2[:, :, 126:], k[:, :, 126:], v[:, :, 126:])

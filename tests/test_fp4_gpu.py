@@ -374,3 +374,22 @@ def test_calls_back_to_back(h3, M):
         per = 2 if M > 8 else 1
         assert all(torch.equal(o, want[i // per % 6]) for i, o in enumerate(got))
     assert h3.load().h3_device_error() == 0
+
+
+def test_offsets_past_32_bits(h3):
+    """Matrices of more than 2^31 elements: the last rows come out as on their own."""
+    x = torch.zeros(420000, 5120, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, 5120, device=DEV).bfloat16()
+    q = h3.quantize_fp4(x, "nvfp4")
+    tail = h3.dequantize_fp4(q)[-3:].clone()
+    assert torch.equal(tail, h3.dequantize_fp4(h3.quantize_fp4(x[-3:].clone(), "nvfp4")))
+    del q, x
+    w = _weight(h3, 27648, 64, "mxfp4", 8)
+    x = torch.randn(80000, 64, device=DEV).bfloat16()
+    y = h3.linear_fp4(x, w)                          # 2.2e9 results, in tiles
+    h3.load().h3_fp4_variant(2)
+    try:
+        assert torch.equal(y[-300:], h3.linear_fp4(x[-300:].clone(), w))
+    finally:
+        h3.load().h3_fp4_variant(0)
+    assert h3.load().h3_device_error() == 0
