@@ -543,57 +543,58 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             ok = mbar_wait(&empty[u % C::STAGES], (u / C::STAGES) & 1, abort_flag);
         }
     } else if (warp == 1 && rank == 0) {
-        // the whole warp runs this; one lane issues
+        // The whole warp runs this and one lane issues, from uniform registers: descriptors are
+        // sums of one per operand, tensor memory addresses constants (all 512 columns are
+        // this CTA's, so they start at 0), and one commit signals both CTAs.
         const uint32_t base = smem_u32(smem);
+        const uint64_t desc_a = smem_desc_sw128(base, 16, 1024), desc_sf = smem_desc_rows16(base + C::OFF_SFA);
+        constexpr uint32_t SF_STEP = C::SF_BYTES >> 4, CHUNK_STEP = CHUNK >> 4;
+        uint32_t slot = 0, phase = 0;                  // of this K tile, then of the two before it
+        uint32_t slot1 = 0, phase1 = 0, slot2 = 0, phase2 = 0;
         uint32_t it = 0, lt = 0;
-        bool ok = true;
+        bool ok = tmem == 0;
         for (int tile = first; tile < num_tiles && ok; tile += step, ++lt) {
             // the accumulator two tiles back has been read wholly before the last one's shared columns
             if (lt > 0) ok = __all_sync(0xffffffffu, mbar_wait_cluster(acc_free, (lt - 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d = tmem + ((lt & 1) ? C::ACC1 : 0);
+            const uint32_t d = (lt & 1) ? C::ACC1 : 0;
             for (int kt = 0; kt < p.ktiles; ++kt, ++it) {
-                const uint32_t slot = it % C::STAGES;
-                ok = mbar_wait(&full[slot], (it / C::STAGES) & 1, abort_flag);
+                ok = mbar_wait(&full[slot], phase, abort_flag);
                 // two scale buffers: the MMAs two K tiles back must have read this one
-                if (ok && it >= 2)
-                    ok = mbar_wait(&empty[(it - 2) % C::STAGES], ((it - 2) / C::STAGES) & 1, abort_flag);
+                if (ok && it >= 2) ok = mbar_wait(&empty[slot2], phase2, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t sa = base + slot * C::STAGE, sb = sa + C::OFF_B;
-                const uint32_t ta = tmem + C::SF_COL0 + (it & 1) * C::SF_COLS, tb = ta + 4 * C::CH;
-                const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
+                const uint64_t at = (slot * C::STAGE) >> 4;
+                const uint64_t da = desc_a + at, db = da + (C::OFF_B >> 4), ds = desc_sf + at;
+                const uint32_t ta = C::SF_COL0 + (it & 1) * C::SF_COLS, tb = ta + 4 * C::CH;
+                const int steps = p.ksteps - kt * (BK / KSTEP);
+                const uint32_t more = kt > 0;
                 if (elect_one()) {
 #pragma unroll
                     for (int c = 0; c < C::CH; ++c) {
                         // w's two 128-row chunks lie side by side: 8 columns per K chunk
-                        tmem_cp_scales<true>(ta + 4 * c, smem_desc_rows16(sa + C::OFF_SFA + c * CHUNK));
-                        tmem_cp_scales<true>(tb + 8 * c, smem_desc_rows16(sa + C::OFF_SFB + c * CHUNK));
-                        tmem_cp_scales<true>(tb + 8 * c + 4,
-                                             smem_desc_rows16(sa + C::OFF_SFB + C::SF_BYTES + c * CHUNK));
+                        tmem_cp_scales<true>(ta + 4 * c, ds + c * CHUNK_STEP);
+                        tmem_cp_scales<true>(tb + 8 * c, ds + SF_STEP + c * CHUNK_STEP);
+                        tmem_cp_scales<true>(tb + 8 * c + 4, ds + 2 * SF_STEP + c * CHUNK_STEP);
                     }
 #pragma unroll
                     for (int s = 0; s < BK / KSTEP; ++s) {
                         const int c = FMT == MX ? s >> 1 : s;
                         if (s < steps)
-                            umma_fp4<FMT == MX, true>(d, smem_desc_sw128(sa + s * 32, 16, 1024),
-                                                      smem_desc_sw128(sb + s * 32, 16, 1024),
+                            umma_fp4<FMT == MX, true>(d, da + 2 * s, db + 2 * s,
                                                       idesc_fp4(256, TILE, FMT == MX, FMT == MX ? (s & 1) * 2 : 0),
-                                                      ta + 4 * c, tb + 8 * c, (kt > 0 || s > 0) ? 1u : 0u);
+                                                      ta + 4 * c, tb + 8 * c, s > 0 ? 1u : more);
                     }
-                    umma_commit_pair(smem_u32(&empty[slot]));
-                    umma_commit_pair(mapa_shared(&empty[slot], 1));
+                    umma_commit_both(&empty[slot]);
+                    if (kt == p.ktiles - 1) umma_commit_both(acc_full);
                 }
                 __syncwarp();
+                slot2 = slot1, phase2 = phase1;
+                slot1 = slot, phase1 = phase;
+                if (++slot == C::STAGES) slot = 0, phase ^= 1;
             }
-            if (!ok) break;
-            if (elect_one()) {
-                umma_commit_pair(smem_u32(acc_full));
-                umma_commit_pair(mapa_shared(acc_full, 1));
-            }
-            __syncwarp();
         }
         if (!ok) drain_in_flight();
     } else if (warp >= 4) {

@@ -307,6 +307,15 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar) {
                  : "memory");
 }
 
+// the same on the mbarriers at this one's offset in both CTAs of the pair
+__device__ __forceinline__ void umma_commit_both(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+
 // Block-scaled 4-bit forms: A and B hold e2m1 codes two a byte, K-major, 64 K elements
 // (32 bytes) per instruction; the scales sit in tensor memory, row r%32 + 32j of the
 // operand in lane r%32, column j, one byte per block.  MXF4: blocks of 32, power-of-two
