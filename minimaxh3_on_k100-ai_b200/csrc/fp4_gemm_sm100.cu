@@ -69,8 +69,8 @@ struct Swap {
     static constexpr int SF_BYTES = CH * CHUNK;
     static constexpr int STAGE = A_BYTES + B_BYTES + 2 * SF_BYTES;
     static constexpr int STAGE_PAD = (STAGE + 1023) / 1024 * 1024;
-    static constexpr int BUDGET = 110 * 1024;                 // two CTAs per SM
-    static constexpr int STAGES = BUDGET / STAGE_PAD;
+    static constexpr int RING_SPACE = 110 * 1024;                 // two CTAs per SM
+    static constexpr int STAGES = RING_SPACE / STAGE_PAD;
     static constexpr int RED_BYTES = BN * 128 * 4;            // the fp32 tile, in the ring's place
     static constexpr int OFF_BAR = STAGES * STAGE_PAD > RED_BYTES ? STAGES * STAGE_PAD : RED_BYTES;
     static constexpr int SMEM = OFF_BAR + (2 * STAGES + 1) * 8 + 16 + 1024;
