@@ -50,7 +50,9 @@ class Fp4Tensor:
     """A matrix of ``rows`` x ``cols`` 4-bit values: ``codes`` uint8
     [rows, ceil(cols/32)*16] (two codes a byte) and ``scales`` uint8
     [ceil(rows/128), ceil(blocks/4), 512], as the products read them.  Immutable but for
-    its contents: the descriptors the entry points take are made once."""
+    its contents: the descriptors the entry points take are made once.  They hold addresses,
+    so a copy (``copy``, ``pickle``, ``torch.save``) takes the tensors and makes its own
+    (``torch.load`` builds this class with ``weights_only=False``)."""
 
     __slots__ = ("rows", "cols", "format", "tensor_scale", "d_codes", "d_scales", "_buffer", "_codes", "_scales")
 
@@ -68,20 +70,36 @@ class Fp4Tensor:
     def _uninitialised(cls, like: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
         """On ``like``'s device, codes and scales in one allocation."""
         pitch, groups, chunks = _layout(rows, cols, format)
-        buf = like.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)
-        at = buf.data_ptr()
-        return cls._of(buf, packed_bytes(at, (rows, pitch), (pitch, 1)),
+        return cls._within(like.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8), rows, cols, format,
+                           tensor_scale)
+
+    @classmethod
+    def _within(cls, buffer: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
+        """Of a buffer that holds the codes, then the scales."""
+        _check_format(format)
+        scale = _check_tensor_scale(format, tensor_scale)
+        pitch, groups, chunks = _layout(rows, cols, format)
+        if buffer.dtype != torch.uint8 or buffer.shape != (rows * pitch + groups * chunks * 512,) or buffer.stride(0) != 1:
+            raise ValueError(f"not the bytes of a {format} matrix [{rows}, {cols}]")
+        at = buffer.data_ptr()
+        return cls._of(buffer, packed_bytes(at, (rows, pitch), (pitch, 1)),
                        packed_bytes(at + rows * pitch, (groups, chunks, 512), (chunks * 512, 512, 1)), rows, cols,
-                       format, tensor_scale)
+                       format, scale)
 
     @classmethod
     def _of(cls, buffer, d_codes, d_scales, rows, cols, format, tensor_scale) -> Fp4Tensor:
-        """Of a buffer laid out as ``_uninitialised`` does."""
+        """Of a buffer laid out as ``_within`` takes it, with its descriptors."""
         self = cls.__new__(cls)
         self._buffer, self.d_codes, self.d_scales, self.rows, self.cols = buffer, d_codes, d_scales, rows, cols
         self.format, self.tensor_scale = format, tensor_scale
         self._codes = self._scales = None
         return self
+
+    def __reduce__(self):
+        rest = (self.rows, self.cols, self.format, self.tensor_scale)
+        if self._buffer is self._codes:      # given as two tensors
+            return Fp4Tensor, (self._codes, self._scales, *rest)
+        return Fp4Tensor._within, (self._buffer, *rest)
 
     @property
     def codes(self) -> torch.Tensor:
