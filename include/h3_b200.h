@@ -338,6 +338,7 @@ int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tenso
  * 16-byte aligned, any contents, at least as many bytes as x's codes and scales together)
  * and multiplied with the 4-bit weight [N,K] of the same format; fp32 accumulation, one
  * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1.
+ * The tensor scales' product has to be below 2^128 (fp32), so not both may be 2^64.
  * y may not overlap an input.  With a NULL workspace (at most 8 rows, N at most 8388480) the product quantises x itself, in one launch;
  * the results are those of form 1 of h3_fp4_variant. */
 int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace, const h3_tensor *w_codes,

@@ -827,6 +827,8 @@ int check_product(const h3_tensor *y, const h3_tensor *xc, const h3_tensor *xs, 
         if (outs > 1 && bias->strides[0] != 1) return H3_ERR_BAD_LAYOUT;
     }
     if (!tensor_scale_ok(fmt, tx) || !tensor_scale_ok(fmt, tw)) return H3_ERR_UNSUPPORTED;
+    p->t = tx * tw;
+    if (isinf(p->t)) return H3_ERR_UNSUPPORTED;      // 0 times it would be NaN
     if (rows > 0x3fffffffLL || outs > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
     p->M = (int)rows;
     p->N = (int)outs;
@@ -838,7 +840,6 @@ int check_product(const h3_tensor *y, const h3_tensor *xc, const h3_tensor *xs, 
     p->y = static_cast<__nv_bfloat16 *>(y->data);
     p->ldy = rows > 1 ? y->strides[0] : 0;
     p->bias = bias && outs > 0 ? static_cast<const __nv_bfloat16 *>(bias->data) : nullptr;
-    p->t = tx * tw;
     p->wide = aligned_to(y->data, 8) && p->ldy % 4 == 0;
     return H3_OK;
 }

@@ -154,6 +154,11 @@ def fp4_tensor_scale(amax: float) -> float:
     return 2.0 ** max(-64, min(64, e - 1 if m == 0.5 else e))
 
 
+def _check_scales_together(x_scale: float, w_scale: float) -> None:
+    if x_scale * w_scale >= 2.0 ** 128:
+        raise ValueError(f"the tensor scales {x_scale} and {w_scale} multiply to more than fp32 holds")
+
+
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
     return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
 
@@ -267,7 +272,7 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
     """out [..., N] BF16 = x W^T (+ bias), both in ``weight``'s 4-bit format, fp32
     accumulation, one rounding.  ``x`` BF16 [..., K] is quantised on the way in (with
     ``x_tensor_scale`` for nvfp4), or given as an ``Fp4Tensor`` (then out is [M, N]) when
-    several projections share it."""
+    several projections share it.  The product of the two tensor scales has to be below 2^128."""
     o2 = _rows_to_write(out)
     if isinstance(x, Fp4Tensor):
         require_cuda(out, x._buffer, weight._buffer, bias)
@@ -275,6 +280,7 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
             raise ValueError(f"x is {x.format}, the weight {weight.format}")
         if x.cols != weight.cols:
             raise ValueError(f"x has {x.cols} columns, the weight {weight.cols}")
+        _check_scales_together(x.tensor_scale, weight.tensor_scale)
         call("h3_linear_fp4_quantized", packed(o2), x.d_codes, x.d_scales, weight.d_codes, weight.d_scales,
              packed(bias), x.cols, _FORMAT[weight.format], x.tensor_scale, weight.tensor_scale, stream_of(out))
         return out
@@ -284,6 +290,7 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
         raise ValueError(f"x has {cols} columns, the weight {weight.cols}")
     require_cuda(out, x, weight._buffer, bias)
     scale = _check_tensor_scale(weight.format, x_tensor_scale)
+    _check_scales_together(scale, weight.tensor_scale)
     work = None
     if rows > FUSED_ROWS:
         pitch, groups, chunks = _layout(rows, cols, weight.format)

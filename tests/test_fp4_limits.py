@@ -1,0 +1,69 @@
+"""The ends of the 4-bit projections' ranges: tensor scales."""
+import ctypes
+
+import pytest
+import torch
+
+DEV = "cuda"
+H3_ERR_UNSUPPORTED = 5
+
+
+@pytest.fixture(scope="module")
+def h3():
+    import h3b200
+    return h3b200
+
+
+def _bf16(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def test_scales_that_overflow_together_are_refused_by_the_entry_points(h3):
+    """2^64 times 2^64 is infinite in fp32, and a sum of 0 times that NaN.  (A weight without
+    rows: what is accepted has nothing to do.)"""
+    lib, d = h3.load(), h3._lib.desc
+    x, w, y = _bf16(4, 48), h3.fp4_empty(0, 48, "nvfp4", device="cpu"), _bf16(4, 0)
+    xq, work = h3.fp4_empty(4, 48, "nvfp4", device="cpu"), torch.zeros(1024, dtype=torch.uint8)
+
+    def status(tx, tw, quantized, workspace=work):
+        ref = lambda t: None if t is None else ctypes.byref(d(t))  # noqa: E731
+        if quantized:
+            return lib.h3_linear_fp4_quantized(*[ref(t) for t in (y, xq.codes, xq.scales, w.codes, w.scales, None)], 48,
+                                               1, tx, tw, None)
+        return lib.h3_linear_fp4(*[ref(t) for t in (y, x, workspace, w.codes, w.scales, None)], 1, tx, tw, None)
+
+    for args in ((True,), (False,), (False, None)):
+        assert status(2.0 ** 64, 2.0 ** 64, *args) == H3_ERR_UNSUPPORTED
+        assert status(2.0 ** 64, 2.0 ** 63, *args) == 0 and status(2.0 ** 63, 2.0 ** 64, *args) == 0
+        assert status(2.0 ** -64, 2.0 ** -64, *args) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 8, 40, 200, 1000])
+def test_largest_and_smallest_scales(h3, M):
+    """Products at the ends of the range: rows of zeros give the bias, and a single product
+    (code 6 times code 6 at the block scale that keeps it in fp32) is rounded once."""
+    bias = torch.randn(300, device=DEV).bfloat16()
+    for tx, tw, block in ((2.0 ** 64, 2.0 ** 63, 2.0 ** -9), (2.0 ** 63, 2.0 ** 64, 2.0 ** -9),
+                          (2.0 ** -64, 2.0 ** -64, 448.0)):
+        x, weight = torch.zeros(M, 64, device=DEV), torch.zeros(300, 64, device=DEV)
+        x[:, 5], weight[:, 5] = 6 * block * tx, 6 * block * tw
+        w = h3.quantize_fp4(weight.bfloat16(), "nvfp4", tw)
+        zeros = torch.zeros(M, 64, device=DEV).bfloat16()
+        for rows, value in ((zeros, None), (x.bfloat16(), (6 * block) ** 2 * tx * tw)):
+            want = bias.expand(M, -1) if value is None else torch.full((M, 300), value, device=DEV).bfloat16()
+            add = bias if value is None else None
+            assert torch.equal(h3.linear_fp4(rows, w, add, x_tensor_scale=tx), want)
+            assert torch.equal(h3.linear_fp4(h3.quantize_fp4(rows, "nvfp4", tx), w, add), want)
+    assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_scales_that_overflow_together_are_refused(h3):
+    w = h3.fp4_empty(64, 64, "nvfp4", 2.0 ** 64)
+    for M in (4, 40):
+        x = torch.zeros(M, 64, dtype=torch.bfloat16, device=DEV)
+        with pytest.raises(ValueError, match="multiply"):
+            h3.linear_fp4(x, w, x_tensor_scale=2.0 ** 64)
+        with pytest.raises(ValueError, match="multiply"):
+            h3.linear_fp4(h3.quantize_fp4(x, "nvfp4", 2.0 ** 64), w)
