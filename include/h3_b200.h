@@ -192,8 +192,10 @@ int h3_mha_scatter(const h3_tensor *dsts, int32_t ndst, const h3_tensor *q, cons
  * number of states of each sample (clamped to [0, Sk]), or NULL for Sk.  Non-causal,
  * fp32 softmax and accumulation, P rounded to BF16.  States behind a sample's length are
  * not read into a result whatever they hold; a sample without states, and a row whose
- * scores are all -inf, gets zeros.  out may not overlap k or v.  scale positive and finite.  Layout rules of h3_mha.
+ * scores are all -inf, gets zeros.  out may not overlap k or v.  scale positive, at most
+ * H3_CROSS_SCALE_MAX.  Layout rules of h3_mha.
  * No reference counterpart (its attention, h3_mha, has one key length and equal heads). */
+#define H3_CROSS_SCALE_MAX 2.3e38f   /* times log2(e) it is still an fp32 number */
 int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, const h3_tensor *v,
                        const h3_tensor *lengths, float scale, void *stream);
 

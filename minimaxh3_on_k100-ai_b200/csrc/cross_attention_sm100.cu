@@ -1022,7 +1022,7 @@ extern "C" int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, cons
         if (lengths->ndim != 1 || lengths->shape[0] != B) return H3_ERR_BAD_SHAPE;
         if (B > 1 && lengths->strides[0] != 1) return H3_ERR_BAD_LAYOUT;
     }
-    if (!(scale > 0.f) || !(scale <= 3.0e38f)) return H3_ERR_UNSUPPORTED;
+    if (!(scale > 0.f) || !(scale <= H3_CROSS_SCALE_MAX)) return H3_ERR_UNSUPPORTED;
     if (numel(q) == 0) return H3_OK;
     cross::Params p{};
     p.B = (int)B;

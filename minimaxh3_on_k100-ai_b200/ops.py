@@ -188,6 +188,9 @@ def mha(q, k, v, scale=None):
     return mha_(torch.empty(q.shape, dtype=q.dtype, device=q.device), q, k, v, scale)
 
 
+CROSS_SCALE_MAX = 2.3e38     # times log2(e) it is still an fp32 number
+
+
 def cross_attention_(out, q, k, v, lengths=None, scale=None):
     """Attention of q [B,Sq,H,D] to an encoder's states k, v [B or 1,Sk,Hkv,D] of another
     length, into out [B,Sq,H,D] (D = 128, H a multiple of Hkv).  ``lengths`` [B] int64 on
@@ -197,8 +200,8 @@ def cross_attention_(out, q, k, v, lengths=None, scale=None):
     require_cuda(out, q, k, v, lengths)
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    if not 0.0 < scale <= 3e38:
-        raise ValueError(f"the scale must be positive and finite, got {scale}")
+    if not 0.0 < scale <= CROSS_SCALE_MAX:
+        raise ValueError(f"the scale must be positive and at most {CROSS_SCALE_MAX}, got {scale}")
     call("h3_cross_attention", packed(out), packed(q), packed(k), packed(v), packed(lengths), scale, stream_of(q))
     return out
 

@@ -1,0 +1,48 @@
+"""The ends of the cross attention's ranges: scales and scores that fp32 cannot hold."""
+import ctypes
+
+import pytest
+import torch
+
+DEV = "cuda"
+H3_ERR_UNSUPPORTED = 5
+
+
+@pytest.fixture(scope="module")
+def h3():
+    import h3b200
+    return h3b200
+
+
+@pytest.fixture(params=[1, 2], ids=["rows", "tiles"])
+def form(h3, request):
+    old = h3.load().h3_cross_attention_variant(request.param)
+    yield request.param
+    h3.load().h3_cross_attention_variant(old)
+
+
+def test_scales_past_fp32_are_refused_by_the_entry_point(h3):
+    """scale * log2(e) has to be an fp32 number.  (No queries: what is accepted has nothing to do.)"""
+    q, k = torch.zeros(1, 0, 2, 128, dtype=torch.bfloat16), torch.zeros(1, 3, 2, 128, dtype=torch.bfloat16)
+    ref = [ctypes.byref(h3._lib.desc(t)) for t in (q, q, k, k)]
+
+    def status(scale):
+        return h3.load().h3_cross_attention(*ref, None, scale, None)
+
+    assert status(2.36e38) == status(3.0e38) == status(3.4e38) == H3_ERR_UNSUPPORTED
+    assert status(2.3e38) == status(1e-40) == 0
+
+
+@pytest.mark.gpu
+def test_the_largest_scale(h3, form):
+    """A score of zero times the largest scale is zero: the mean of the states."""
+    for Sq in (1, 40, 200):
+        q = torch.zeros(1, Sq, 2, 128, device=DEV).bfloat16()
+        kv = torch.randn(1, 64, 2, 2, 128, device=DEV).bfloat16()
+        out = h3.cross_attention(q, kv[:, :, 0], kv[:, :, 1], scale=2.3e38)
+        # every weight is 1 before the division: 64 fp32 additions, a division by 64, one rounding
+        mean, size = kv[:, :, 1].double().mean(1), kv[:, :, 1].double().abs().mean(1)
+        assert bool(((out.double() - mean[:, None]).abs() <= 2.0 ** -8 * mean.abs() + 64 * 2.0 ** -23 * size).all())
+        for scale in (2.36e38, 3e38):
+            with pytest.raises(ValueError, match="scale"):
+                h3.cross_attention(q, kv[:, :, 0], kv[:, :, 1], scale=scale)
