@@ -438,7 +438,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 named_bar_sync(1 + t, 128);
             }
             const float lsum = l0 + l1;
-            const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;       // no state, or none with a finite score
+            // No state, or none with a finite score: zeros.  A maximum that fp32 cannot hold: NaN (the
+            // fused product minus it is -inf for every finite score, which would read as no state).
+            const float inv = m == INFINITY ? NAN : lsum == 0.f ? 0.f : 1.0f / lsum;
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
                 uint32_t o[32];

@@ -46,3 +46,30 @@ def test_the_largest_scale(h3, form):
         for scale in (2.36e38, 3e38):
             with pytest.raises(ValueError, match="scale"):
                 h3.cross_attention(q, kv[:, :, 0], kv[:, :, 1], scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Sq,Sk", [(1, 9), (4, 300), (30, 1000), (200, 40), (300, 700)])
+def test_scores_past_fp32_show_as_nan(h3, form, Sq, Sk):
+    """A scaled score above fp32's largest number makes its row NaN (infinity minus infinity),
+    wherever it lies among the keys; rows of the same tile whose scores fit are not touched."""
+    q = torch.rand(1, Sq, 2, 128, device=DEV).bfloat16()
+    kv = torch.rand(1, Sk, 2, 2, 128, device=DEV).bfloat16()
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    want = h3.cross_attention(q, k, v, scale=1e-3)
+    big = q.clone()
+    big[:, ::3] = 1e16                          # scores of about 6e17: times 1e25 they overflow
+    small = (q.float() * 1e-28).bfloat16()      # and of these the scaled scores are below 1
+    mixed = torch.where(torch.arange(Sq, device=DEV).view(1, -1, 1, 1) % 3 == 0, big, small)
+    out = h3.cross_attention(mixed, k, v, scale=1e25)
+    assert bool(out[:, ::3].isnan().all())
+    rest = torch.ones(Sq, dtype=torch.bool, device=DEV)
+    rest[::3] = False
+    assert torch.equal(out[:, rest], h3.cross_attention(small, k, v, scale=1e25)[:, rest])
+    assert not bool(out[:, rest].isnan().any())
+    # one key at the end does it too
+    k = k.clone()
+    k[:, -1] = 1e30
+    out = h3.cross_attention(q, k, v, scale=1e9)
+    assert bool(out.isnan().all())
+    assert not bool(want.isnan().any()) and h3.load().h3_device_error() == 0
