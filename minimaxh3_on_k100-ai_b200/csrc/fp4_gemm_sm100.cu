@@ -780,7 +780,7 @@ std::atomic<int> g_variant{0};
 // 512 x 5120 x 5120 swap 20.1, tiles 15.9; 777 x 5120 x 5120 swap 21.4, tiles 26.7.
 template <int FMT>
 bool swap_form(const Params &p) {
-    if ((p.N + 127) / 128 > 65535) return false;     // its grid's limit
+    if ((p.N + 127) / 128 > 65535 || (p.M + 127) / 128 > 65535) return false;     // its grid's limits
     if (p.M <= 128) return true;
     const int64_t tiles = (int64_t)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
     const int64_t small = (int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128);

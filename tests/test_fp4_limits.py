@@ -67,3 +67,23 @@ def test_scales_that_overflow_together_are_refused(h3):
             h3.linear_fp4(x, w, x_tensor_scale=2.0 ** 64)
         with pytest.raises(ValueError, match="multiply"):
             h3.linear_fp4(h3.quantize_fp4(x, "nvfp4", 2.0 ** 64), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("M", [65535 * 128 + 1, 65535 * 128 + 777])
+def test_more_rows_than_the_swap_form_has_blocks_for(h3, fmt, M):
+    """Rows of x past 65535 blocks of 128: any count is taken.  A row's result is the one it
+    has among fewer rows (in the tile form, which adds in the same order whatever the size)."""
+    N, K = 24, 32
+    w = h3.quantize_fp4((torch.randn(N, K, device=DEV) * 0.02).bfloat16(), fmt)
+    bias = torch.randn(N, device=DEV).bfloat16()
+    x = torch.randn(M, K, device=DEV).bfloat16()
+    y = h3.linear_fp4(x, w, bias)
+    old = h3.load().h3_fp4_variant(2)
+    try:
+        for at in (0, M // 2, M - 500):
+            assert torch.equal(y[at:at + 500], h3.linear_fp4(x[at:at + 500], w, bias))
+    finally:
+        h3.load().h3_fp4_variant(old)
+    assert h3.load().h3_device_error() == 0
