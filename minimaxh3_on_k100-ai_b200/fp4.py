@@ -25,7 +25,8 @@ __all__ = ["Fp4Tensor", "FP4_BLOCK", "fp4_empty", "fp4_tensor_scale", "quantize_
 
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _FORMAT = {"mxfp4": 0, "nvfp4": 1}
-FUSED_ROWS = 8       # up to so many rows the product quantises x itself, without a workspace
+FUSED_ROWS = 8       # up to so many rows the product quantises x itself, without a workspace,
+FUSED_OUTS = 65535 * 128    # for up to so many rows of the weight (its grid's limit)
 
 
 def _check_format(fmt: str) -> int:
@@ -267,6 +268,10 @@ def unpack_fp4(q: Fp4Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 # ---------------------------------------------------------------------------
 # projection
 # ---------------------------------------------------------------------------
+def _fused_rows(weight: Fp4Tensor) -> int:
+    return FUSED_ROWS if weight.rows <= FUSED_OUTS else 0
+
+
 def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tensor | None = None,
                 x_tensor_scale: float = 1.0) -> torch.Tensor:
     """out [..., N] BF16 = x W^T (+ bias), both in ``weight``'s 4-bit format, fp32
@@ -292,7 +297,7 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
     scale = _check_tensor_scale(weight.format, x_tensor_scale)
     _check_scales_together(scale, weight.tensor_scale)
     work = None
-    if rows > FUSED_ROWS:
+    if rows > _fused_rows(weight):
         pitch, groups, chunks = _layout(rows, cols, weight.format)
         work = x.new_empty(rows * pitch + groups * chunks * 512, dtype=torch.uint8)   # x in 4 bits
     call("h3_linear_fp4", packed(o2), packed(x2), packed(work), weight.d_codes, weight.d_scales, packed(bias),
@@ -306,7 +311,7 @@ def linear_fp4(x: torch.Tensor | Fp4Tensor, weight: Fp4Tensor, bias: torch.Tenso
     if host() and not isinstance(x, Fp4Tensor):
         out = host().linear_fp4(x, weight._buffer, weight.d_codes, weight.d_scales, weight.rows, weight.cols, bias,
                                 _FORMAT[weight.format], _check_tensor_scale(weight.format, x_tensor_scale),
-                                weight.tensor_scale, FUSED_ROWS)
+                                weight.tensor_scale, _fused_rows(weight))
         if out is not None:
             CALLS["n"] += 1
             return out

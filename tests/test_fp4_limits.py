@@ -87,3 +87,28 @@ def test_more_rows_than_the_swap_form_has_blocks_for(h3, fmt, M):
     finally:
         h3.load().h3_fp4_variant(old)
     assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_few_rows_by_more_outputs_than_the_fused_form_takes(h3, monkeypatch):
+    """A weight of more than 65535 blocks of 128 rows, and so few rows of x that they would be
+    quantised inside the product: any count of outputs is taken, through either way of
+    calling.  An output is the one of its weight row among fewer (one instruction covers K)."""
+    N, K = 65535 * 128 + 1, 16
+    w = h3.quantize_fp4((torch.randn(N, K, device=DEV) * 0.02).bfloat16(), "nvfp4")
+    codes, scales = h3.unpack_fp4(w)
+    tail = h3.pack_fp4(codes[-600:], scales[-600:], "nvfp4", cols=K)
+    bias = torch.randn(N, device=DEV).bfloat16()
+    for M in (1, 8):
+        x = torch.randn(M, K, device=DEV).bfloat16()
+        old = h3.load().h3_fp4_variant(2)
+        want = h3.linear_fp4(h3.quantize_fp4(x), tail, bias[-600:])
+        h3.load().h3_fp4_variant(old)
+        for fast in (True, False):
+            with monkeypatch.context() as m:
+                if not fast:
+                    m.setattr(h3._lib, "_host", False)
+                y = h3.linear_fp4(x, w, bias)
+            assert y.shape == (M, N) and torch.equal(y[:, -600:], want)
+    assert h3.linear_fp4(x[:0], w, bias).shape == (0, N)
+    assert h3.load().h3_device_error() == 0
