@@ -327,6 +327,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         if (!ok) drain_in_flight();
     } else if (((warp - 4) >> 2) < NQ) {
         // ------------------------------------------------------------ softmax, output
+        // The group's warps find out one by one that a wait gave up, and one may still pass a wait
+        // that another gave up on.  So `ok` decides only what a warp computes: each passes both
+        // named barriers of every item to the end.
         const int t = (warp - 4) >> 2;
         const int row = (warp & 3) * 32 + lane;
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
@@ -341,7 +344,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             item_at(item, b, h, q0, len);
             const int nkv = (len + BN - 1) / BN;
             float m = -INFINITY, l0 = 0.f, l1 = 0.f;
-            for (int j = 0; j < nkv; ++j, ++n) {
+            int j = 0;
+            for (; j < nkv && ok; ++j, ++n) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], n & 1, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
@@ -428,21 +432,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 tc_fence_before();
                 mbar_arrive(&p_ready[t]);
             }
-            if (!ok) break;
-            if (nkv > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (n - 1) & 1, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-            } else {
+            if (j == 0) {                        // no states, or given up before the barrier of the first tile
                 if (row == 0) tma_store_wait_read();
                 named_bar_sync(1 + t, 128);
+            } else if (ok) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (n - 1) & 1, abort_flag));
+                tc_fence_after();
             }
             const float lsum = l0 + l1;
             // No state, or none with a finite score: zeros.  A maximum that fp32 cannot hold: NaN (the
             // fused product minus it is -inf for every finite score, which would read as no state).
             const float inv = m == INFINITY ? NAN : lsum == 0.f ? 0.f : 1.0f / lsum;
 #pragma unroll 1
-            for (int cc = 0; cc < 4; ++cc) {
+            for (int cc = 0; cc < 4 && ok; ++cc) {
                 uint32_t o[32];
                 if (nkv > 0) {
                     tmem_ld32(o_addr + cc * 32, o);
@@ -462,7 +464,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             tc_fence_before();
             fence_proxy_async_smem();
             named_bar_sync(1 + t, 128);
-            if (row == 0 && q0 + t * BM < p.Sq) {                    // rows past Sq are clipped
+            // rows past Sq are clipped; where a warp gave up its rows are not there
+            if (row == 0 && q0 + t * BM < p.Sq && !*abort_flag) {
                 tma_store_4d(&to, p_ptr, 0, q0 + t * BM, h, b);
                 tma_store_4d(&to, p_ptr + HALF, 64, q0 + t * BM, h, b);
                 tma_store_commit();
