@@ -517,11 +517,12 @@ __device__ __forceinline__ void fa_cta(const CUtensorMap &tq, const CUtensorMap 
                 named_bar_sync(1 + t, 128);
                 const int c = row & 15;
                 const uint32_t tile = out_tile + (uint32_t)(c >> 3) * HALF;
+                const int end = *abort_flag ? 0 : p.Sq;   // a warp that gave up has left its rows unfinished
 #pragma unroll 4
                 for (int k = 0; k < BM / 8; ++k) {
                     const int rr = (row >> 4) + 8 * k;
                     const int g = q0 + t * BM + rr;
-                    if (g >= p.Sq) break;   // rows grow with k
+                    if (g >= end) break;   // rows grow with k
                     const int dq = g / p.rows_per_dst;
                     const int tl = g - dq * p.rows_per_dst;
                     const uint4 v = ld_shared_v4(tile + swz(rr, c & 7));
@@ -530,7 +531,7 @@ __device__ __forceinline__ void fa_cta(const CUtensorMap &tq, const CUtensorMap 
             } else {
                 fence_proxy_async_smem();
                 named_bar_sync(1 + t, 128);
-                if (row == 0 && q0 + t * BM < p.Sq) {
+                if (row == 0 && q0 + t * BM < p.Sq && !*abort_flag) {
                     tma_store_4d(&to, sQ + t * TILE, 0, q0 + t * BM, h, b);
                     tma_store_4d(&to, sQ + t * TILE + HALF, 64, q0 + t * BM, h, b);
                     tma_store_commit();
@@ -538,7 +539,10 @@ __device__ __forceinline__ void fa_cta(const CUtensorMap &tq, const CUtensorMap 
                 }
             }
         } else {
+            // another warp of the group may still have passed the wait this one gave up on: it
+            // stands at the barrier above, which takes all four
             drain_in_flight();
+            named_bar_sync(1 + t, 128);
         }
     }
 

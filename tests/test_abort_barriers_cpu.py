@@ -87,8 +87,9 @@ static void group(const int warp, const int lane) {
     uint32_t tmem = 0;
     uint8_t smem[1] = {};
     bool ok = true;
-    (void)ok;
+    {
 %(code)s
+    }
 }
 
 int main() {
@@ -162,3 +163,25 @@ def test_cross_attention_tile_form(tmp_path):
     code = _branch(text, "const int t = (warp - 4) >> 2;")
     for lens in ((300, 0, 128, 0, 0, 129, 1), (0, 500), (77, 0), (1000,)):
         _run(tmp_path, code, lens, CROSS)
+
+
+ATTENTION = r"""
+#define H3_ATTN_MAX_ACC 4
+#define H3_ATTN_MAX_BF16 0
+#define H3_ATTN_EARLY_P %d
+constexpr int O_COL = 256, TILE = TILE_BYTES, SUM_GROUPS = 2, GROUP_PAIRS = 32, POLY_PAIRS = 0;
+struct Params { int Sq, Sk, ndst, rows_per_dst; float scale_log2; int64_t d_row, d_head; __nv_bfloat16 *dst[1]; };
+static Params p = {1 << 20, 0, 0, 1 << 20, 1.f};
+static int to, nkv;
+static const int q0 = 0, h = 0, b = 0;
+static uint8_t sQ[1 << 17], sP[1 << 17];
+// number of key tiles, and whether the rows go to one tensor or to their owners
+static void set_mode(int m) { p.ndst = m %% 2, nkv = m / 2 + 1, p.Sk = nkv * BN; }
+"""
+
+
+@pytest.mark.parametrize("early_p", [0, 1])
+def test_self_attention(tmp_path, early_p):
+    text = (CSRC / "attention_sm100.cu").read_text()
+    code = _branch(text, "const int t = (warp - 4) >> 2;")
+    _run(tmp_path, code, (0,), ATTENTION % early_p, modes=8)
