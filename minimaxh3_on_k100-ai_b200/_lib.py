@@ -9,12 +9,15 @@ import ctypes
 import importlib.util
 import os
 import struct
+import warnings
 from pathlib import Path
 
 import torch
 
+from .build import host_path
+
 LIB_PATH = Path(__file__).resolve().parent / "libh3b200.so"
-HOST_PATH = LIB_PATH.with_name("_h3host.so")
+HOST_PATH = host_path()
 
 H3_OK = 0
 _STATUS = {
@@ -192,18 +195,22 @@ def host():
     """The extension that makes the regular calls of the small-launch operators without
     ctypes (csrc/host_calls.cpp), bound to this library's entry points.  Its functions
     return None for whatever is not in order; the caller then goes through ``call``, whose
-    checks raise.  False where it was not built: every call then goes through ``call``."""
+    checks raise.  False where it was not built for this Python and torch, or does not load
+    (which warns, once): every call then goes through ``call``."""
     global _host
     if _host is None:
+        _host = False
         if HOST_PATH.exists():
-            spec = importlib.util.spec_from_file_location("_h3host", HOST_PATH)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
             lib = load()
-            module.bind(*[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
-            _host = module
-        else:
-            _host = False
+            spec = importlib.util.spec_from_file_location("_h3host", HOST_PATH)
+            try:
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+            except ImportError as e:
+                warnings.warn(f"{HOST_PATH.name} does not load, calls go through ctypes: {e}", RuntimeWarning)
+            else:
+                module.bind(*[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _HOST_ENTRIES])
+                _host = module
     return _host
 
 

@@ -20,7 +20,6 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG.parent / "_build"
 LIB = PKG / "libh3b200.so"
-HOST = PKG / "_h3host.so"      # csrc/host_calls.cpp: the small operators' calls without ctypes
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",
@@ -71,30 +70,37 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     return LIB
 
 
+def host_path() -> Path:
+    """The extension of csrc/host_calls.cpp for this Python and this torch, whose C++ layouts it
+    is compiled against: under another of either it is another file, and built again."""
+    import torch
+    return PKG / f"_h3host.{sys.implementation.cache_tag}-torch{torch.__version__}.so"
+
+
 def build_host(verbose: bool = False) -> Path:
     """The Python extension over torch's C++ headers (the host compiler, no nvcc)."""
     import sysconfig
 
     import torch
-    src = CSRC / "host_calls.cpp"
+    src, out = CSRC / "host_calls.cpp", host_path()
     newest = max(src.stat().st_mtime, (INCLUDE / "h3_b200.h").stat().st_mtime)
-    if HOST.exists() and HOST.stat().st_mtime >= newest:
-        return HOST
+    if out.exists() and out.stat().st_mtime >= newest:
+        return out
     root = Path(torch.__path__[0])
     cuda = Path(_nvcc()).resolve().parent.parent / "include"
     includes = [sysconfig.get_path("include"), root / "include", root / "include/torch/csrc/api/include", cuda]
-    tmp = HOST.with_suffix(".so.tmp")
+    tmp = out.with_suffix(".tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{i}" for i in includes], str(src), "-o", str(tmp), f"-L{root / 'lib'}",
            "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{root / 'lib'}"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"building {HOST.name} failed:\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, HOST)
+        raise RuntimeError(f"building {out.name} failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, out)
     if verbose:
-        print(HOST)
-    return HOST
+        print(out)
+    return out
 
 
 if __name__ == "__main__":
