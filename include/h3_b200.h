@@ -320,8 +320,9 @@ int h3_adaln_projection(const h3_tensor *y, const h3_tensor *x, const h3_tensor 
  *          the low nibble of byte i, 2i+1 in the high one, zero codes past cols;
  *   scales [ceil(rows/128), ceil(blocks/4), 512] contiguous, 16-byte aligned, blocks =
  *          ceil(cols / block size): the scale of row r, block b is byte
- *          (r%32)*16 + (r%128)/32*4 + b%4 of chunk [r/128][b/4].  Blocks past the last
- *          hold 0; rows past the last one may hold anything. */
+ *          (r%32)*16 + (r%128)/32*4 + b%4 of chunk [r/128][b/4], of NVFP4 below 128
+ *          (the products' scales have no sign).  Blocks past the last hold 0; rows
+ *          past the last one may hold anything. */
 
 /* codes, scales = x [rows, cols] BF16 (inner stride 1) in `format`.
  *   MXFP4: scale 2^e, e = clamp(floor(log2 amax) - 2, -127, 127)

@@ -227,7 +227,8 @@ def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, format: str, cols: int |
              tensor_scale: float = 1.0) -> Fp4Tensor:
     """A 4-bit matrix from row-major parts, as checkpoints store them: ``codes`` uint8
     [rows, ceil(cols/2)] (column 2i in the low nibble of byte i) and ``scales`` uint8 (or
-    e4m3) [rows, ceil(cols/block)].  A set-up step: lays the scales out once, in torch."""
+    e4m3, without signs) [rows, ceil(cols/block)].  A set-up step: lays the scales out once, in
+    torch, and looks at them on the host."""
     _check_format(format)
     if scales.dtype != torch.uint8 and scales.element_size() == 1:
         scales = scales.view(torch.uint8)
@@ -244,6 +245,8 @@ def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, format: str, cols: int |
     if cols < 1 or codes.shape[1] != (cols + 1) // 2 or scales.shape[1] != blocks:
         raise ValueError(f"{cols} columns need {(cols + 1) // 2} code bytes and {blocks} scales a row, got "
                          f"{codes.shape[1]} and {scales.shape[1]}")
+    if format == "nvfp4" and bool((scales >= 128).any()):
+        raise ValueError("nvfp4 scales have no sign: their bytes are below 128")
     out = fp4_empty(rows, cols, format, tensor_scale, codes.device)
     out.codes.zero_()
     out.codes[:, : codes.shape[1]] = codes
