@@ -60,7 +60,7 @@ typedef enum h3_dtype {
 /* Microscaled 4-bit formats: blocks of consecutive columns of e2m1 codes share a scale. */
 typedef enum h3_fp4_format {
     H3_MXFP4 = 0,   /* blocks of 32, scale 2^(byte - 127); the tensor scale is 1 */
-    H3_NVFP4 = 1    /* blocks of 16, unsigned e4m3 scale times the tensor scale, a power of two in [2^-64, 2^64] */
+    H3_NVFP4 = 1    /* blocks of 16, unsigned e4m3 scale times the tensor scale in [2^-64, 2^64], a power of two to quantise with */
 } h3_fp4_format;
 
 typedef enum h3_status {
@@ -332,8 +332,8 @@ int h3_adaln_projection(const h3_tensor *y, const h3_tensor *x, const h3_tensor 
 int h3_quantize_fp4(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x, int32_t format,
                     float tensor_scale, void *stream);
 
-/* y [rows, cols] BF16 = the values the codes and scales stand for (exact: at most 6
- * significant bits). */
+/* y [rows, cols] BF16 = the values the codes and scales stand for (at most 6 significant bits
+ * times the tensor scale: exact where that is a power of two, else formed in fp32 and rounded). */
 int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tensor *scales, int32_t format,
                       float tensor_scale, void *stream);
 

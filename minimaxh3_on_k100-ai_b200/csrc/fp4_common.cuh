@@ -10,7 +10,8 @@
 //          copies scales as they lie; blocks past the last one hold 0 and rows past the
 //          last one are never read into a result.
 // mxfp4: blocks of 32, scale 2^(byte-127) (byte 255: NaN).  nvfp4: blocks of 16, scale an
-// unsigned e4m3 (byte 127: NaN) times one power of two of the whole tensor.
+// unsigned e4m3 (byte 127: NaN) times one number of the whole tensor, a power of two where
+// the quantisation is done here.
 #pragma once
 
 #include <cuda.h>
@@ -53,12 +54,13 @@ inline int check_held(const h3_tensor *codes, const h3_tensor *scales, int fmt, 
     return H3_OK;
 }
 
-// a power of two that keeps block scale times tensor scale a normal fp32 number
+// the scale of a matrix that is held: block scale times tensor scale is a normal fp32 number
+inline bool held_scale_ok(int fmt, float t) { return fmt == MX ? t == 1.0f : t >= 0x1p-64f && t <= 0x1p64f; }
+// of one that is quantised: a power of two
 inline bool tensor_scale_ok(int fmt, float t) {
     uint32_t u;
     memcpy(&u, &t, 4);
-    if (fmt == MX) return u == 0x3f800000u;
-    return (u & 0x807fffffu) == 0 && t >= 0x1p-64f && t <= 0x1p64f;
+    return held_scale_ok(fmt, t) && (u & 0x007fffffu) == 0;
 }
 
 // ---------------------------------------------------------------------------

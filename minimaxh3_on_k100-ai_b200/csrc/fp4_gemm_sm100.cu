@@ -826,7 +826,7 @@ int check_product(const h3_tensor *y, const h3_tensor *xc, const h3_tensor *xs, 
         if (bias->ndim != 1 || bias->shape[0] != outs) return H3_ERR_BAD_SHAPE;
         if (outs > 1 && bias->strides[0] != 1) return H3_ERR_BAD_LAYOUT;
     }
-    if (!tensor_scale_ok(fmt, tx) || !tensor_scale_ok(fmt, tw)) return H3_ERR_UNSUPPORTED;
+    if (!held_scale_ok(fmt, tx) || !held_scale_ok(fmt, tw)) return H3_ERR_UNSUPPORTED;
     p->t = tx * tw;
     if (isinf(p->t)) return H3_ERR_UNSUPPORTED;      // 0 times it would be NaN
     if (rows > 0x3fffffffLL || outs > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
@@ -873,6 +873,7 @@ extern "C" int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_te
     H3_CHECK(check_bf16(x));
     if (x->ndim != 2 || x->shape[1] < 1) return H3_ERR_BAD_SHAPE;
     if (format != fp4::MX && format != fp4::NV) return H3_ERR_UNSUPPORTED;
+    if (!fp4::tensor_scale_ok(format, x_tensor_scale)) return H3_ERR_UNSUPPORTED;
     const int64_t rows = x->shape[0], cols = x->shape[1];
     if (rows > 0x3fffffffLL || cols > (1 << 24)) return H3_ERR_UNSUPPORTED;
     if ((cols > 1 && x->strides[1] != 1) || (rows > 1 && x->strides[0] < 0)) return H3_ERR_BAD_LAYOUT;

@@ -159,7 +159,7 @@ __device__ __forceinline__ void value_unit(const uint8_t *codes, const uint8_t *
         uint32_t h;
         asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
         const float2 f = __half22float2(*reinterpret_cast<__half2 *>(&h));
-        // 2 significant bits times 4: exact in BF16
+        // 2 significant bits times 4: exact in BF16 where the tensor scale is a power of two
         w[i] = bf2u(__floats2bfloat162_rn(f.x * scale, f.y * scale));
     }
 }
@@ -205,7 +205,7 @@ int plan(const h3_tensor *x, const h3_tensor *codes, const h3_tensor *scales, in
     H3_CHECK(check_bf16(x));
     if (x->ndim != 2 || x->shape[1] < 1) return H3_ERR_BAD_SHAPE;
     H3_CHECK(check_held(codes, scales, fmt, x->shape[0], x->shape[1]));
-    if (!tensor_scale_ok(fmt, tensor_scale)) return H3_ERR_UNSUPPORTED;
+    if (!held_scale_ok(fmt, tensor_scale)) return H3_ERR_UNSUPPORTED;
     if (x->shape[0] > 0x7fffffffLL || x->shape[1] > (1 << 24)) return H3_ERR_UNSUPPORTED;
     if (x->shape[0] == 0) return H3_OK;
     if ((x->shape[1] > 1 && x->strides[1] != 1) || (x->shape[0] > 1 && x->strides[0] < 0)) return H3_ERR_BAD_LAYOUT;
@@ -248,6 +248,7 @@ int quantize(const h3_tensor *codes, const h3_tensor *scales, const h3_tensor *x
     dim3 grid;
     bool vec;
     H3_CHECK(plan(x, codes, scales, fmt, tensor_scale, &s, &grid, &vec));
+    if (!tensor_scale_ok(fmt, tensor_scale)) return H3_ERR_UNSUPPORTED;
     if (x->shape[0] == 0) return H3_OK;
     auto kernel = fmt == MX ? (vec ? quantize_kernel<MX, true> : quantize_kernel<MX, false>)
                             : (vec ? quantize_kernel<NV, true> : quantize_kernel<NV, false>);

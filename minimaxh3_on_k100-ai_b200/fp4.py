@@ -4,8 +4,9 @@ A block of consecutive columns of a row shares one scale; a value is an e2m1 cod
 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times that scale:
 
 * ``"mxfp4"``: blocks of 32, the scale a power of two;
-* ``"nvfp4"``: blocks of 16, the scale an e4m3 number times ``tensor_scale``, one power
-  of two for the whole matrix (``fp4_tensor_scale`` gives one that fits).
+* ``"nvfp4"``: blocks of 16, the scale an e4m3 number times ``tensor_scale``, one number
+  for the whole matrix: a power of two for what is quantised here (``fp4_tensor_scale``
+  gives one that fits), any fp32 number for what a checkpoint brings.
 
 Weights are held as ``Fp4Tensor`` (made once, by ``quantize_fp4`` from BF16 or by
 ``pack_fp4`` from a checkpoint's codes and scales); ``linear_fp4`` quantises its
@@ -14,6 +15,7 @@ No counterpart in the reference.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -36,15 +38,28 @@ def _check_format(fmt: str) -> int:
         raise ValueError(f"unknown 4-bit format {fmt!r}: 'mxfp4' or 'nvfp4'") from None
 
 
-def _check_tensor_scale(fmt: str, scale: float) -> float:
+def _check_held_scale(fmt: str, scale: float) -> float:
+    """The scale of a matrix, as fp32."""
     scale = float(scale)
     if scale == 1.0:
         return scale
+    scale = ctypes.c_float(scale).value
     if fmt == "mxfp4":
         raise ValueError("mxfp4 has no tensor scale")
-    if not (2.0 ** -64 <= scale <= 2.0 ** 64) or math.frexp(scale)[0] != 0.5:
-        raise ValueError(f"the tensor scale must be a power of two in [2^-64, 2^64], got {scale}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        raise ValueError(f"the tensor scale must lie in [2^-64, 2^64], got {scale}")
     return scale
+
+
+def _check_tensor_scale(fmt: str, scale: float) -> float:
+    """The scale of what is quantised here."""
+    scale = float(scale)
+    if scale == 1.0:
+        return scale
+    held = _check_held_scale(fmt, scale)
+    if held != scale or math.frexp(held)[0] != 0.5:
+        raise ValueError(f"the tensor scale must be a power of two to quantise with it, got {scale}")
+    return held
 
 
 class Fp4Tensor:
@@ -61,7 +76,7 @@ class Fp4Tensor:
                  tensor_scale: float = 1.0):
         _check_format(format)
         self.rows, self.cols, self.format = rows, cols, format
-        self.tensor_scale = _check_tensor_scale(format, tensor_scale)
+        self.tensor_scale = _check_held_scale(format, tensor_scale)
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
         self._codes, self._scales, self._buffer = codes, scales, codes
@@ -78,7 +93,7 @@ class Fp4Tensor:
     def _within(cls, buffer: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
         """Of a buffer that holds the codes, then the scales."""
         _check_format(format)
-        scale = _check_tensor_scale(format, tensor_scale)
+        scale = _check_held_scale(format, tensor_scale)
         pitch, groups, chunks = _layout(rows, cols, format)
         if buffer.dtype != torch.uint8 or buffer.shape != (rows * pitch + groups * chunks * 512,) or buffer.stride(0) != 1:
             raise ValueError(f"not the bytes of a {format} matrix [{rows}, {cols}]")
@@ -156,7 +171,7 @@ def fp4_tensor_scale(amax: float) -> float:
 
 
 def _check_scales_together(x_scale: float, w_scale: float) -> None:
-    if x_scale * w_scale >= 2.0 ** 128:
+    if math.isinf(ctypes.c_float(x_scale * w_scale).value):
         raise ValueError(f"the tensor scales {x_scale} and {w_scale} multiply to more than fp32 holds")
 
 
@@ -175,8 +190,9 @@ def _rows_to_write(out: torch.Tensor) -> torch.Tensor:
 # quantisation
 # ---------------------------------------------------------------------------
 def quantize_fp4_(out: Fp4Tensor, x: torch.Tensor) -> Fp4Tensor:
-    """Quantise x [..., cols] BF16 into ``out`` (its format and tensor scale)."""
+    """Quantise x [..., cols] BF16 into ``out`` (its format and tensor scale, a power of two)."""
     require_cuda(out._buffer, x)
+    _check_tensor_scale(out.format, out.tensor_scale)
     x2 = _rows_of(x)
     if x2.shape != (out.rows, out.cols):
         raise ValueError(f"x has shape {tuple(x2.shape)}, the 4-bit matrix {out.shape}")
@@ -213,7 +229,8 @@ def dequantize_fp4_(out: torch.Tensor, q: Fp4Tensor) -> torch.Tensor:
 
 
 def dequantize_fp4(q: Fp4Tensor) -> torch.Tensor:
-    """The values a 4-bit matrix stands for, [rows, cols] BF16 (exact)."""
+    """The values a 4-bit matrix stands for, [rows, cols] BF16: exact, but rounded where the
+    tensor scale is no power of two."""
     if host():
         out = host().dequantize_fp4(q._buffer, q.d_codes, q.d_scales, q.rows, q.cols, _FORMAT[q.format],
                                     q.tensor_scale)
@@ -247,7 +264,7 @@ def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, format: str, cols: int |
                          f"{codes.shape[1]} and {scales.shape[1]}")
     if format == "nvfp4" and bool((scales >= 128).any()):
         raise ValueError("nvfp4 scales have no sign: their bytes are below 128")
-    out = fp4_empty(rows, cols, format, tensor_scale, codes.device)
+    out = Fp4Tensor._uninitialised(codes, rows, cols, format, tensor_scale)
     out.codes.zero_()
     out.codes[:, : codes.shape[1]] = codes
     if cols % 2:

@@ -90,7 +90,7 @@ def test_bytes_that_do_not_fit_are_refused(h3):
     q = _packed(h3, "nvfp4")
     rebuild, args = q.__reduce__()
     for bad in ((args[0][:-1], *args[1:]), (args[0].view(2, -1), *args[1:]), (args[0].int(), *args[1:]),
-                (args[0], args[1] + 1, *args[2:]), (*args[:3], "int4", 1.0), (*args[:4], 3.0)):
+                (args[0], args[1] + 1, *args[2:]), (*args[:3], "int4", 1.0), (*args[:4], 2.0 ** 65)):
         with pytest.raises(ValueError):
             rebuild(*bad)
 
