@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster spans grid x
-    const int n0 = (int)blockIdx.y * 128, m0 = (int)blockIdx.z * BN;
+    const int n0 = (int)blockIdx.y * 128, m0 = (int)blockIdx.z * BN;   // m0: a multiple of 128 (0 where BN is smaller)
     const int k_begin = (int)((int64_t)p.ktiles * rank / split), k_end = (int)((int64_t)p.ktiles * (rank + 1) / split);
     const int nk = k_end - k_begin;
 
@@ -205,7 +205,6 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
             const uint32_t ta = tmem + C::SF_COL0 + (i & 1) * 2 * C::SF_COLS, tb = ta + C::SF_COLS;
             const int ch = min(C::CH, p.chunks - kt * C::CH);
             const int steps = min(BK / KSTEP, p.ksteps - kt * (BK / KSTEP));
-            const uint32_t tb0 = tb + ((m0 & 127) >> 5);     // this tile's rows within the 128-row chunk
             if (elect_one()) {
 #pragma unroll
                 for (int c = 0; c < C::CH; ++c) {
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(SWAP_THREADS + (FUSED ? QUANT_WARPS * 32 : 0),
                         umma_fp4<FMT == MX, false>(tmem, smem_desc_sw128(sa + s * 32, 16, 1024),
                                                    smem_desc_sw128(sb + s * 32, 16, 1024),
                                                    idesc_fp4(128, BN, FMT == MX, FMT == MX ? (s & 1) * 2 : 0),
-                                                   ta + 4 * c, tb0 + 4 * c, (i > 0 || s > 0) ? 1u : 0u);
+                                                   ta + 4 * c, tb + 4 * c, (i > 0 || s > 0) ? 1u : 0u);
                 }
                 umma_commit(&empty[slot]);
                 if (i == nk - 1) umma_commit(done);
