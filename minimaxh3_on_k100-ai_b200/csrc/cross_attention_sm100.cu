@@ -71,7 +71,7 @@ struct Params {
 
 __device__ __forceinline__ int states(const Params &p, int b) {
     if (!p.lens) return p.Sk;
-    const int64_t n = __ldg(p.lens + b);
+    const int64_t n = p.lens[b];
     return n < 0 ? 0 : n > p.Sk ? p.Sk : (int)n;
 }
 

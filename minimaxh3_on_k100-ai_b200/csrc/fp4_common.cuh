@@ -82,16 +82,16 @@ __device__ __forceinline__ float rcp(float x) {
 template <bool VEC>
 __device__ __forceinline__ void load_unit(const __nv_bfloat16 *row, int col, int cols, uint32_t (&w)[8]) {
     if (VEC && col + UNIT <= cols) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(row + col));
-        const uint4 b = __ldg(reinterpret_cast<const uint4 *>(row + col) + 1);
+        const uint4 a = reinterpret_cast<const uint4 *>(row + col)[0];
+        const uint4 b = reinterpret_cast<const uint4 *>(row + col)[1];
         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
         w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     } else {
         const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t lo = col + 2 * i < cols ? __ldg(p + col + 2 * i) : 0;
-            const uint32_t hi = col + 2 * i + 1 < cols ? __ldg(p + col + 2 * i + 1) : 0;
+            const uint32_t lo = col + 2 * i < cols ? p[col + 2 * i] : 0;
+            const uint32_t hi = col + 2 * i + 1 < cols ? p[col + 2 * i + 1] : 0;
             w[i] = lo | (hi << 16);
         }
     }

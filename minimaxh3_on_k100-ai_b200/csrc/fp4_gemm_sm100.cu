@@ -621,8 +621,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 uint16_t b0 = 0, b1 = 0;
                 if (p.bias) {
                     const uint16_t *b = reinterpret_cast<const uint16_t *>(p.bias) + col + 2 * lane;
-                    if (col + 2 * lane < p.N) b0 = __ldg(b);
-                    if (col + 2 * lane + 1 < p.N) b1 = __ldg(b + 1);
+                    if (col + 2 * lane < p.N) b0 = b[0];
+                    if (col + 2 * lane + 1 < p.N) b1 = b[1];
                 }
                 tmem_ld_wait();
                 if (i == 0) {

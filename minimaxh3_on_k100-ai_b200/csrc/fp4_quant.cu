@@ -49,7 +49,7 @@ __device__ __forceinline__ void load_segment(uint16_t *seg, const __nv_bfloat16 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int k = t + i * tx;
-        if (k >= a && k < inside) v[i] = __ldg(words + k);
+        if (k >= a && k < inside) v[i] = words[k];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -57,8 +57,8 @@ __device__ __forceinline__ void load_segment(uint16_t *seg, const __nv_bfloat16 
         if (k >= a && k < inside) dst[k] = v[i];
     }
     if (t == 0) {
-        if (a) seg[1] = __ldg(p);
-        if ((n + a) & 1) seg[n - 1 + a] = __ldg(p + n - 1);
+        if (a) seg[1] = p[0];
+        if ((n + a) & 1) seg[n - 1 + a] = p[n - 1];
     }
 }
 // one thread's 16 elements of the copy
@@ -146,10 +146,10 @@ __global__ void __launch_bounds__(THREADS)
 template <int FMT>
 __device__ __forceinline__ void value_unit(const uint8_t *codes, const uint8_t *scales, const Shape &s, int64_t row,
                                            int unit, uint32_t (&w)[8]) {
-    const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes + row * s.ldc + unit * (UNIT / 2)));
+    const uint2 c = *reinterpret_cast<const uint2 *>(codes + row * s.ldc + unit * (UNIT / 2));
     const int block = FMT == MX ? unit >> 1 : unit;
-    const uint32_t byte = __ldg(scales + ((row >> 7) * s.chunks + (block >> 2)) * CHUNK + (row & 31) * 16 +
-                                ((row >> 5) & 3) * 4 + (block & 3));
+    const uint32_t byte = scales[((row >> 7) * s.chunks + (block >> 2)) * CHUNK + (row & 31) * 16 +
+                                 ((row >> 5) & 3) * 4 + (block & 3)];
     float scale;
     if (FMT == MX) scale = byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte == 0 ? 1u << 22 : byte << 23);
     else scale = from_e4m3(byte) * s.ts.t;      // cvt makes byte 127 a NaN

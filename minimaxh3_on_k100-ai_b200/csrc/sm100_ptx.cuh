@@ -134,7 +134,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 // Programmatic dependent launch: a kernel launched with overlapped_launch() is set up while
 // the one before it in its stream drains, and calls wait_for_previous() before it touches
 // memory that may be that kernel's (all of it is visible afterwards); release_next() lets
-// the kernel after it start its set-up already.
+// the kernel after it start its set-up already.  Such a kernel reads with plain loads: the
+// read-only ones (__ldg) are for memory that nothing writes while the kernel lives, which
+// here begins before the wait, and a compiler may move them ahead of it.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
