@@ -52,7 +52,7 @@ struct Params {
     const __nv_bfloat16 *bias;   // may be null
     float t;
     int num_m, num_n;            // tiles
-    int wide;                    // 4-column (8-byte) stores allowed
+    int wide;                    // 4-column (8-byte) stores allowed; tile form: stores through TMA
     int dependent;               // launched behind the quantisation of x: w may be read before that ends
     // fused quantisation: x itself
     const __nv_bfloat16 *x;
@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        tma_store_2d(&ty, buf, col, row0);               // clipped at y's edges
+                        tma_store_2d(&ty, buf, col, row0);               // clipped at y's last row and column
                         tma_store_commit();
                     }
                 } else {
@@ -738,11 +738,13 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
     p.num_m = (p.M + TILE - 1) / TILE;
     p.num_n = (p.N + TILE - 1) / TILE;
     if ((int64_t)p.num_m * p.num_n > 0x3fffffff) return H3_ERR_UNSUPPORTED;
-    p.wide = aligned16(p.y) && p.ldy % 8 == 0;
+    // a store through TMA is cut off at y's last row exactly, but along a row at 16 bytes only: rows
+    // of whole 16 bytes, or the columns beside y's would be written
+    p.wide = aligned16(p.y) && p.ldy % 8 == 0 && p.N % 8 == 0;
     CUtensorMap ty = tx;                             // not used where rows are too odd for it
     if (p.wide) {
         const cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M};
-        const cuuint64_t strides[1] = {(cuuint64_t)(p.M > 1 ? p.ldy : (p.N + 7) / 8 * 8) * 2};
+        const cuuint64_t strides[1] = {(cuuint64_t)(p.M > 1 ? p.ldy : p.N) * 2};
         const cuuint32_t box[2] = {64, 32};
         H3_CHECK(make_tmap_bf16(&ty, p.y, 2, dims, strides, box));
     }
