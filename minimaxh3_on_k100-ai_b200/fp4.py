@@ -70,7 +70,8 @@ class Fp4Tensor:
     so a copy (``copy``, ``pickle``, ``torch.save``) takes the tensors and makes its own
     (``torch.load`` builds this class with ``weights_only=False``)."""
 
-    __slots__ = ("rows", "cols", "format", "tensor_scale", "d_codes", "d_scales", "_buffer", "_codes", "_scales")
+    __slots__ = ("rows", "cols", "format", "tensor_scale", "d_codes", "d_scales", "_buffer", "_held_scales", "_codes",
+                 "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, format: str,
                  tensor_scale: float = 1.0):
@@ -79,8 +80,11 @@ class Fp4Tensor:
         self.tensor_scale = _check_held_scale(format, tensor_scale)
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
-        self._codes, self._scales, self._buffer = codes, scales, codes
-        self.d_codes, self.d_scales = packed(codes), packed(scales)
+        # tensors of its own over the same memory: what is given may be pointed elsewhere (a
+        # Parameter that moves with its module), and these keep the memory described here alive
+        self._buffer, self._held_scales = codes.detach(), scales.detach()
+        self._codes = self._scales = None
+        self.d_codes, self.d_scales = packed(self._buffer), packed(self._held_scales)
 
     @classmethod
     def _uninitialised(cls, like: torch.Tensor, rows: int, cols: int, format: str, tensor_scale: float) -> Fp4Tensor:
@@ -108,27 +112,29 @@ class Fp4Tensor:
         self = cls.__new__(cls)
         self._buffer, self.d_codes, self.d_scales, self.rows, self.cols = buffer, d_codes, d_scales, rows, cols
         self.format, self.tensor_scale = format, tensor_scale
-        self._codes = self._scales = None
+        self._held_scales = self._codes = self._scales = None
         return self
 
     def __reduce__(self):
         rest = (self.rows, self.cols, self.format, self.tensor_scale)
-        if self._buffer is self._codes:      # given as two tensors
-            return Fp4Tensor, (self._codes, self._scales, *rest)
+        if self._held_scales is not None:    # given as two tensors
+            return Fp4Tensor, (self._buffer, self._held_scales, *rest)
         return Fp4Tensor._within, (self._buffer, *rest)
 
     @property
     def codes(self) -> torch.Tensor:
         if self._codes is None:
             pitch, _, _ = _layout(self.rows, self.cols, self.format)
-            self._codes = self._buffer[: self.rows * pitch].view(self.rows, pitch)
+            self._codes = (self._buffer[: self.rows * pitch].view(self.rows, pitch) if self._held_scales is None
+                           else self._buffer.detach())
         return self._codes
 
     @property
     def scales(self) -> torch.Tensor:
         if self._scales is None:
             pitch, groups, chunks = _layout(self.rows, self.cols, self.format)
-            self._scales = self._buffer[self.rows * pitch:].view(groups, chunks, 512)
+            self._scales = (self._buffer[self.rows * pitch:].view(groups, chunks, 512) if self._held_scales is None
+                            else self._held_scales.detach())
         return self._scales
 
     @property

@@ -111,3 +111,26 @@ def test_a_copy_outlives_the_original(h3, fmt, way):
         # quantising into the copy leaves the original's bytes
         h3.quantize_fp4_(c, values)
         assert bool((q.codes == 0x77).all())
+
+
+def test_what_it_was_made_of_may_be_pointed_elsewhere(h3):
+    """A Parameter that moves with its module gets other memory under the same object; the
+    matrix keeps the memory that its descriptors name, and the device of it."""
+    made = _packed(h3, "nvfp4")
+    codes, scales = (torch.nn.Parameter(t.clone(), requires_grad=False) for t in (made.codes, made.scales))
+    q = h3.Fp4Tensor(codes, scales, made.rows, made.cols, "nvfp4", made.tensor_scale)
+    assert _addresses(q) == (codes.data_ptr(), scales.data_ptr())
+    codes[0, 0] = 0x55                                    # contents are shared
+    assert int(q.codes[0, 0]) == 0x55
+    want = q.codes.clone()
+    for t in (codes, scales, q.codes, q.scales):
+        t.data = torch.zeros_like(t)
+    assert _addresses(q)[0] == q._buffer.data_ptr() and torch.equal(q._buffer, want)
+    assert _addresses(q)[1] == q._held_scales.data_ptr()
+    c = copy.deepcopy(q)
+    assert torch.equal(c.codes, want) and torch.equal(c.scales, made.scales)
+    module = torch.nn.Module()
+    module.codes, module.scales = (torch.nn.Parameter(t.clone(), requires_grad=False) for t in (made.codes, made.scales))
+    q = h3.Fp4Tensor(module.codes, module.scales, made.rows, made.cols, "nvfp4", made.tensor_scale)
+    module.to("meta")
+    assert module.codes.device.type == "meta" and q.device.type == "cpu" and torch.equal(q.codes, made.codes)
