@@ -1,4 +1,5 @@
-"""The ends of the cross attention's ranges: scales and scores that fp32 cannot hold."""
+"""The ends of the cross attention's ranges: scales and scores that fp32 cannot hold, the
+result in the queries' place, many samples."""
 import ctypes
 
 import pytest
@@ -73,3 +74,37 @@ def test_scores_past_fp32_show_as_nan(h3, form, Sq, Sk):
     out = h3.cross_attention(q, k, v, scale=1e9)
     assert bool(out.isnan().all())
     assert not bool(want.isnan().any()) and h3.load().h3_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_into_the_queries(h3, form):
+    """The result may take the queries' place."""
+    for B, Sq, Sk, H, Hkv in ((2, 1, 300, 8, 2), (3, 40, 500, 4, 4), (1, 5, 5000, 8, 8), (2, 300, 200, 4, 2),
+                              (1, 3001, 300, 4, 4)):
+        q = torch.randn(B, Sq, H, 128, device=DEV).bfloat16()
+        kv = torch.randn(B, Sk, 2, Hkv, 128, device=DEV).bfloat16()
+        want = h3.cross_attention(q, kv[:, :, 0], kv[:, :, 1])
+        for _ in range(3):
+            z = q.clone()
+            assert h3.cross_attention_(z, z, kv[:, :, 0], kv[:, :, 1]) is z
+            assert torch.equal(z, want)
+    assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [511, 512, 513, 2000])
+@pytest.mark.parametrize("Sq", [1, 150])
+def test_sample_counts_around_what_is_sorted(h3, form, B, Sq):
+    """Up to 512 samples are dealt by their length, more as they come.  (P rounds to BF16 and the
+    result does, 2^-8 each; 2^-15 for the scores and sums in fp32.)"""
+    q = torch.randn(B, Sq, 2, 128, device=DEV).bfloat16()
+    kv = torch.randn(B, 200, 2, 1, 128, device=DEV).bfloat16()
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    lengths = torch.randint(0, 201, (B,), device=DEV)
+    out = h3.cross_attention(q, k, v, lengths)
+    s = torch.einsum("bqhd,bkd->bhqk", q.double(), k[:, :, 0].double()) * 128 ** -0.5
+    s.masked_fill_((torch.arange(200, device=DEV) >= lengths[:, None])[:, None, None], float("-inf"))
+    w = torch.softmax(s, -1).nan_to_num(0.0)                       # a sample without states: zeros
+    ref, mag = (torch.einsum("bhqk,bkd->bqhd", w, t) for t in (v[:, :, 0].double(), v[:, :, 0].double().abs()))
+    assert bool(((out.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -8 + 2.0 ** -15) * mag).all())
+    assert h3.load().h3_device_error() == 0

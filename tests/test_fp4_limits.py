@@ -1,4 +1,4 @@
-"""The ends of the 4-bit projections' ranges: tensor scales."""
+"""The ends of the 4-bit projections' ranges: tensor scales, rows, outputs and columns."""
 import ctypes
 
 import pytest
@@ -111,4 +111,25 @@ def test_few_rows_by_more_outputs_than_the_fused_form_takes(h3, monkeypatch):
                 y = h3.linear_fp4(x, w, bias)
             assert y.shape == (M, N) and torch.equal(y[:, -600:], want)
     assert h3.linear_fp4(x[:0], w, bias).shape == (0, N)
+    assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_the_longest_sums(h3, fmt):
+    """K = 2^24 columns, the most there may be, in both forms and quantised inside; one more is
+    refused.  (K/64 instructions with 2^-22 each, 9 more for the join; one rounding to BF16.)"""
+    K = 1 << 24
+    x, w = (torch.randn(n, K, device=DEV).bfloat16() for n in (2, 3))
+    xq, wq = h3.quantize_fp4(x, fmt), h3.quantize_fp4(w, fmt)
+    xv, wv = (h3.dequantize_fp4(q).double() for q in (xq, wq))
+    ref, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    bound = ref.abs() * 2.0 ** -8 + (K / 64 + 9) * 2.0 ** -22 * mag
+    for form in (0, 1, 2):
+        old = h3.load().h3_fp4_variant(form)
+        for y in (h3.linear_fp4(x, wq), h3.linear_fp4(xq, wq)):
+            assert bool(((y.double() - ref).abs() <= bound).all())
+        h3.load().h3_fp4_variant(old)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        h3.quantize_fp4(torch.zeros(1, K + 1, dtype=torch.bfloat16, device=DEV), fmt)
     assert h3.load().h3_device_error() == 0

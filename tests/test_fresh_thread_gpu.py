@@ -2,8 +2,8 @@
 
 Such a thread has no CUDA context bound to it until its first launch, and the descriptors
 of the kernels' TMA copies are made before that.  Each operator is the first thing a new
-thread does, eagerly and into a graph that the thread captures; the result is the main
-thread's, bit for bit.
+thread does, eagerly and into a capture that the main thread began; the result is the main
+thread's, bit for bit.  Beside that: threads that share a stream, and streams that join.
 """
 import threading
 
@@ -97,4 +97,66 @@ def test_first_call_of_a_thread_into_a_capture(h3, name):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+    assert h3.load().h3_device_error() == 0
+
+
+def test_threads_on_one_stream(h3):
+    """Calls of several threads interleave on one stream, a product's quantisation and the
+    product itself among them; each keeps its own rows."""
+    ws = [h3.quantize_fp4((torch.randn(700, 1100, device=DEV) * 0.1).bfloat16(), f) for f in ("nvfp4", "mxfp4") * 2]
+    xs = [torch.randn(m, 1100, device=DEV).bfloat16() for m in (3, 40, 300, 1000)]
+    want = [h3.linear_fp4(x, w) for x, w in zip(xs, ws)]
+    back = [h3.dequantize_fp4(h3.quantize_fp4(x)) for x in xs]
+    torch.cuda.synchronize()
+    wrong, errors = [0] * len(xs), []
+
+    def run(i):
+        try:
+            for _ in range(100):
+                y, d = h3.linear_fp4(xs[i], ws[i]), h3.dequantize_fp4(h3.quantize_fp4(xs[i]))
+                wrong[i] += not (torch.equal(y, want[i]) and torch.equal(d, back[i]))
+        except Exception as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and wrong == [0] * len(xs)
+    assert h3.load().h3_device_error() == 0
+
+
+@pytest.mark.parametrize("M", [3, 100, 700])
+def test_weights_written_on_another_branch_of_a_capture(h3, M):
+    """The product reads its weights ahead of the quantisation's end; here they are written on a
+    stream that joins just before."""
+    x = torch.randn(M, 1100, device=DEV).bfloat16()
+    w = (torch.randn(640, 1100, device=DEV) * 0.1).bfloat16()
+    want = h3.linear_fp4(x, h3.quantize_fp4(w))
+    wq, inp, side, graph = h3.fp4_empty(640, 1100), torch.zeros_like(x), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    wq.codes.zero_(), wq.scales.zero_()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            h3.quantize_fp4_(wq, w)
+        rows = inp * 1.0
+        held = h3.quantize_fp4(rows)
+        here.wait_stream(side)
+        y, z = h3.linear_fp4(rows, wq), h3.linear_fp4(held, wq)
+    inp.copy_(x)
+    for _ in range(3):
+        wq.codes.zero_()
+        graph.replay()
+        assert torch.equal(y, want)
+        assert torch.equal(z, h3.linear_fp4(h3.quantize_fp4(x), wq))
+    # the same without a capture
+    for _ in range(20):
+        wq.codes.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            h3.quantize_fp4_(wq, w)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(h3.linear_fp4(x, wq), want)
     assert h3.load().h3_device_error() == 0
