@@ -60,7 +60,8 @@ typedef enum h3_dtype {
 /* Microscaled 4-bit formats: blocks of consecutive columns of e2m1 codes share a scale. */
 typedef enum h3_fp4_format {
     H3_MXFP4 = 0,   /* blocks of 32, scale 2^(byte - 127); the tensor scale is 1 */
-    H3_NVFP4 = 1    /* blocks of 16, unsigned e4m3 scale times the tensor scale in [2^-64, 2^64], a power of two to quantise with */
+    H3_NVFP4 = 1    /* blocks of 16, unsigned e4m3 scale times the tensor scale in [2^-64, 2^64],
+                     * which has to be a power of two to quantise with */
 } h3_fp4_format;
 
 typedef enum h3_status {
@@ -71,7 +72,7 @@ typedef enum h3_status {
     H3_ERR_BAD_LAYOUT = 4,    /* strides/alignment the op cannot address         */
     H3_ERR_UNSUPPORTED = 5,   /* valid request outside what this build supports  */
     H3_ERR_LAUNCH = 6,        /* the CUDA launch reported an error               */
-    H3_ERR_DRIVER = 7,        /* a driver entry point could not be resolved      */
+    H3_ERR_DRIVER = 7,        /* a driver entry point is missing or failed       */
     H3_ERR_TIMEOUT = 8,       /* a bounded device-side wait gave up              */
     H3_ERR_INDEX = 9,         /* a row index was outside the indexed tensor      */
     H3_ERR_TOO_LARGE = 10     /* request exceeds the library's static scratch    */
@@ -192,8 +193,9 @@ int h3_mha_scatter(const h3_tensor *dsts, int32_t ndst, const h3_tensor *q, cons
  * number of states of each sample (clamped to [0, Sk]), or NULL for Sk.  Non-causal,
  * fp32 softmax and accumulation, P rounded to BF16.  States behind a sample's length are
  * not read into a result whatever they hold; a sample without states, and a row whose
- * scores are all -inf, gets zeros.  out may not overlap k or v.  scale positive, at most
- * H3_CROSS_SCALE_MAX.  Layout rules of h3_mha.
+ * scores are all -inf, gets zeros; a scaled score past fp32 makes its row NaN.  out may be q,
+ * and else overlap no input.  scale positive, at most H3_CROSS_SCALE_MAX.  At most 65535
+ * samples and heads.  Layout rules of h3_mha: a batch stride of 0 for k and v, both, only.
  * No reference counterpart (its attention, h3_mha, has one key length and equal heads). */
 #define H3_CROSS_SCALE_MAX 2.3e38f   /* times log2(e) it is still an fp32 number */
 int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, const h3_tensor *k, const h3_tensor *v,
@@ -342,8 +344,9 @@ int h3_dequantize_fp4(const h3_tensor *y, const h3_tensor *codes, const h3_tenso
  * and multiplied with the 4-bit weight [N,K] of the same format; fp32 accumulation, one
  * rounding.  bias [N] BF16 or NULL.  Any M, N, K >= 1 (K at most 2^24); inner strides 1.
  * The tensor scales' product has to be below 2^128 (fp32), so not both may be 2^64.
- * y may not overlap an input.  With a NULL workspace (at most 8 rows, N at most 8388480) the product quantises x itself, in one launch;
- * the results are those of form 1 of h3_fp4_variant. */
+ * y may not overlap an input; what lies beside y in wider rows stays as it was.  With a NULL
+ * workspace (at most 8 rows, N at most 8388480) the product quantises x itself, in one
+ * launch; the results are those of form 1 of h3_fp4_variant. */
 int h3_linear_fp4(const h3_tensor *y, const h3_tensor *x, const h3_tensor *workspace, const h3_tensor *w_codes,
                   const h3_tensor *w_scales, const h3_tensor *bias, int32_t format, float x_tensor_scale,
                   float w_tensor_scale, void *stream);

@@ -27,7 +27,7 @@ _STATUS = {
     4: "bad layout (strides/alignment)",
     5: "unsupported configuration",
     6: "CUDA launch error",
-    7: "driver entry point unavailable",
+    7: "driver entry point unavailable or failed",
     8: "bounded device wait timed out",
     9: "row index outside the indexed tensor",
     10: "request exceeds the library's static scratch capacity",
@@ -176,7 +176,8 @@ def check(status: int, op: str) -> None:
 
 
 # Number of C-ABI entry-point calls made (each launches exactly one kernel, or
-# none for an empty input); bench.py reads it to count its kernel launches.
+# none for an empty input; h3_linear_fp4 with a workspace launches two); bench.py
+# reads it to count its kernel launches, none of which are that entry point's.
 CALLS = {"n": 0}
 
 

@@ -983,8 +983,8 @@ int launch_rows(const h3_tensor *k, const h3_tensor *v, cross::Params &p, cudaSt
 // CTA per SM), 1.45 (16 rows, 64 keys, two) or 1.1 (32 rows, 64 keys); 128 keys of one Q tile
 // 1.47, of two 2.07, and 1.5 to store an item; the rest of a launch 5 to 9.5.  Checked at
 // 16..512 queries, 512..18432 states, 2..640 groups: e.g. 32 queries, 40 heads, 512 states
-// 13.0 us in rows and 11.3 in tiles, 2304 states 22.5 and 29.7; 512 queries of 2 heads over
-// 18432 states 79 and 197.
+// 12.9 us in rows and 10.8 in tiles, 2304 states 23.1 and 31.5; 512 queries of 2 heads over
+// 18432 states 79 and 207.
 bool rows_form(const cross::Params &p, int64_t rows, int64_t groups) {
     const int sms = num_sms();
     const int64_t tiles = (p.Sq + cross::BM - 1) / cross::BM, heads = (int64_t)p.H * p.B;
@@ -1056,8 +1056,8 @@ extern "C" int h3_cross_attention(const h3_tensor *out, const h3_tensor *q, cons
         p.rows = (int)rows;
         if (rows > 16) return launch_rows<2, 4>(k, v, p, (cudaStream_t)stream);
         // Eight warps fill an SM on their own, four leave room for a second CTA.  Measured at one
-        // query, 18432 states, 8 key/value heads (cluster of 16): 18.8 us with eight, 21.6 with four;
-        // at 160 (sample, head) groups of 512 states, more than there are SMs: 16.0 and 11.7 us.
+        // query, 18432 states, 8 key/value heads (clusters of 10): 18.5 us with eight, 21.5 with four;
+        // at 160 (sample, head) groups of 512 states, more than there are SMs: 15.6 and 11.3 us.
         return groups <= num_sms() ? launch_rows<1, 8>(k, v, p, (cudaStream_t)stream)
                                    : launch_rows<1, 4>(k, v, p, (cudaStream_t)stream);
     }

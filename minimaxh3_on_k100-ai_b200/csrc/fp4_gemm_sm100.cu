@@ -13,8 +13,10 @@
 // no scratch in global memory).  Bound by reading the weights (HBM).
 //
 // For up to 8 rows the same kernel can quantise x itself: four more warps write this CTA's
-// share of x to the ring, which saves a launch and the scratch (1 x 15360 x 5120 nvfp4:
-// 13.7 us against 14.3; 16 rows would take 12.9 against 9.6 at 5120 x 5120).
+// share of x to the ring, which saves a launch and the scratch.  nvfp4, back to back in a
+// graph: 1 x 15360 x 5120 11.8 us against 12.8 with the quantisation before it, 4 rows 12.3
+// against 12.6, 8 rows 13.1 against 12.8 (there it is the second launch's host time that is
+// saved); 16 rows would take 16.9 against 13.0.
 //
 // tile form: persistent CTA pairs (cta_group::2), 256 x 256 output tiles, K in tiles of 256
 // (one 128-byte swizzle span of codes) through a 5-slot TMA ring.  Each CTA loads its 128 x
@@ -384,8 +386,8 @@ int swap_split(int64_t tiles, int ktiles) {
     }
     int split = ktiles < 8 ? ktiles : 8;
     // The count takes one CTA per SM, as if each used all of tensor memory; two run (their
-    // columns and shared memory fit).  Measured at 1 x 15360 x 5120 nvfp4: 14.6 us with a
-    // split for one per SM, 12.4 for two.
+    // columns and shared memory fit).  Measured at 1 x 15360 x 5120 nvfp4: 13.3 us with a
+    // split for one per SM, 11.8 for two.
     while (split > 1 && 2 * resident[dev][split].load() < tiles) --split;
     return split;
 }
@@ -432,7 +434,7 @@ constexpr int TILE = 256;                        // rows and columns of a pair's
 constexpr int EPI_WARPS = 8;                     // two per quarter of the rows, each every other 64 columns
 constexpr int TILE_THREADS = (4 + EPI_WARPS) * 32;
 // Column tiles per raster group.  Sustained at 18944 x 27648 x 5120 nvfp4, under the power cap:
-// groups of 4 / 8 / 20 / 32 / 64 / all ran 1385 / 1362 / 1336 / 1328 / 1350 / 1483 us.
+// groups of 4 / 8 / 20 / 32 / 64 / all ran 1331 / 1267 / 1216 / 1206 / 1252 / 1445 us.
 constexpr int GROUP_N = 32;
 
 template <int FMT>
@@ -666,8 +668,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     }
                 } else {
                     // Rows too odd for TMA: two columns per lane, a row at a time.  (4-byte words
-                    // across neighbouring lanes where the row starts half way into one took
-                    // longer: 13.9 us against 11.9 at 333 x 4861 x 1795.)
+                    // across neighbouring lanes where the row starts half way into one took 2 us
+                    // longer at 333 x 4861 x 1795, which runs 11.0; 333 x 4864, through TMA, 9.3.)
                     __syncwarp();
                     const int rows = min(32, p.M - row0), left = p.N - col - 2 * lane;
                     const uint32_t at = smem_u32(buf) + (lane & 3) * 4;
@@ -773,12 +775,14 @@ int launch_tiles(const h3_tensor *xc, const h3_tensor *wc, Params &p, cudaStream
 // 0 chooses per launch, 1 forces the swap form, 2 the tile form (h3_fp4_variant)
 std::atomic<int> g_variant{0};
 
-// Whether the swap form takes less time than the tile form, from times measured on B200
-// (us): a wave of tiles 0.47 per K tile and 1 to hand over, of the swap form's 128 x 128
-// tiles 0.62 per K tile of a CTA's share (0.82 in several waves); the rest of a launch 5.5
-// and 8.  Checked at M 17
-// to 2048, N 1000 to 27648, K 1000 to 13824: e.g. 256 x 5120 x 13824 swap 19.9, tiles 30;
-// 512 x 5120 x 5120 swap 20.1, tiles 15.9; 777 x 5120 x 5120 swap 21.4, tiles 26.7.
+// Whether the swap form takes less time than the tile form, by an estimate (us): a wave of
+// tiles 0.47 per K tile and 1 to hand over, of the swap form's 128 x 128 tiles 0.62 per K tile
+// of a CTA's share (0.82 in several waves); the rest of a launch 5.5 and 8.  Both forms
+// measured at M 129 to 1500 and six N x K from 1000 x 1000 to 27648 x 5120, nvfp4: 256 x 5120
+// x 13824 swap 20.5, tiles 24.1; 512 x 5120 x 5120 swap 19.8, tiles 13.4; 777 x 5120 x 5120
+// swap 20.6, tiles 20.5.  The constants are those of a slower state of the tile form, so the
+// choice keeps to the swap form a little too long: at worst 1.17 times the tiles' time (384 x
+// 5120 x 5120: 15.4 and 13.4; 777 x 4861 x 1795: 16.6 and 14.9), else within 1.07.
 template <int FMT>
 bool swap_form(const Params &p) {
     if ((p.N + 127) / 128 > 65535 || (p.M + 127) / 128 > 65535) return false;     // its grid's limits

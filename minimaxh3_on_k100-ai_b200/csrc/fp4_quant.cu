@@ -33,7 +33,7 @@ struct Shape {
 
 // Rows that 16-byte accesses do not fit (odd widths): the tx threads of a row move its
 // segment of 16 tx elements between global and shared memory by neighbouring 4-byte words
-// instead of each its own unit 32 bytes away from the next thread's (187 -> 27 us to read
+// instead of each its own unit 32 bytes away from the next thread's (187 -> 21 us to read
 // back 18944 x 1795).  The copy in shared memory starts at element `a` (0 or 1) of its
 // space, so that its words are the row's words; n elements exist.
 constexpr int SEG_PAD = 8;               // elements between the segments of a block's rows

@@ -302,8 +302,8 @@ def linear_fp4_(out: torch.Tensor, x: torch.Tensor | Fp4Tensor, weight: Fp4Tenso
                 x_tensor_scale: float = 1.0) -> torch.Tensor:
     """out [..., N] BF16 = x W^T (+ bias), both in ``weight``'s 4-bit format, fp32
     accumulation, one rounding.  ``x`` BF16 [..., K] is quantised on the way in (with
-    ``x_tensor_scale`` for nvfp4), or given as an ``Fp4Tensor`` (then out is [M, N]) when
-    several projections share it.  The product of the two tensor scales has to be below 2^128."""
+    ``x_tensor_scale`` for nvfp4), or given as an ``Fp4Tensor`` (with its own scale; out is
+    then [M, N]) when several projections share it.  The product of the two tensor scales has to be below 2^128."""
     o2 = _rows_to_write(out)
     if isinstance(x, Fp4Tensor):
         require_cuda(out, x._buffer, weight._buffer, bias)
